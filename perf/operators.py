@@ -1,0 +1,505 @@
+"""What the paged 8-bit KV cache's speed is measured on: the steps of a server
+that batches requests of different lengths, through the public entry points of
+``sgq``.
+
+A page holds ``page`` tokens of every kv head, with one fp32 scale per page and
+head for K and one for V: K quants ``[n_pages, n_kv, page, hd]``, V quants
+``[n_pages, n_kv, page/32, hd, 32]`` (each group of 32 tokens transposed), both
+int8, scales ``[n_pages, n_kv]``.
+
+  plan     block tables and the slot map of a step, from the requests' lengths
+           (with the pages of finished requests given back first)
+  append   the step's K and V rows into their pages, and the written blocks
+           read back as values
+  attn     attention of the step's query rows over the pages
+
+The sizes are those of the two decoder geometries the framework is built for
+(32 query heads; head_dim 128 over 16 kv heads, or head_dim 256 / 512 over
+16 / 4) and of its prompt chunks.  The plain forms are batched torch operations
+in fp32 (fp64 for the quantization's borders); ``exact`` computes the same
+outputs in fp64, request by request.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+N_Q = 32
+DEV = "cuda"
+
+
+def listed():
+    return [
+        # a decode step of a busy server: one new token for each of 64 requests
+        {"name": "plan_decode", "kind": "plan", "seqs": 64, "page": 32, "width": 256, "chunk": 0},
+        # a step of a large batch: an eighth of the rows has finished and takes new prompts
+        {"name": "plan_turnover", "kind": "plan", "seqs": 1024, "page": 64, "width": 128,
+         "chunk": 251},
+        # one decoded token of one request: the smallest call, latency
+        {"name": "append_token", "kind": "append", "hd": 128, "n_kv": 16, "page": 32, "f16": False,
+         "seqs": 1, "new": 1},
+        # one token of each of 64 requests, f16 rows
+        {"name": "append_decode", "kind": "append", "hd": 128, "n_kv": 16, "page": 32, "f16": True,
+         "seqs": 64, "new": 1},
+        # a 4096-token prompt chunk, f16 rows
+        {"name": "append_prompt", "kind": "append", "hd": 128, "n_kv": 16, "page": 64, "f16": True,
+         "seqs": 1, "new": 4096},
+        # odd chunks of three requests at a sliding layer's head_dim, fp32 rows
+        {"name": "append_odd", "kind": "append", "hd": 256, "n_kv": 16, "page": 32, "f16": False,
+         "seqs": 3, "new": 777},
+        # one request at an 8K context, fp32 rows as the model driver holds them
+        {"name": "attn_one", "kind": "attn", "hd": 128, "n_kv": 16, "page": 32, "f16": False,
+         "decodes": 1, "prompts": 0, "chunk": 0, "kv": 8191, "window": 0},
+        # 64 requests with 2K to 8K tokens each
+        {"name": "attn_decode", "kind": "attn", "hd": 128, "n_kv": 16, "page": 32, "f16": True,
+         "decodes": 64, "prompts": 0, "chunk": 0, "kv": 8192, "window": 0},
+        # a global layer of the released geometry: 8 query heads share a kv head
+        {"name": "attn_decode_global", "kind": "attn", "hd": 512, "n_kv": 4, "page": 64,
+         "f16": True, "decodes": 12, "prompts": 0, "chunk": 0, "kv": 32768, "window": 0},
+        # two prompts of ordinary odd length from their first token on
+        {"name": "attn_prompt", "kind": "attn", "hd": 128, "n_kv": 16, "page": 64, "f16": True,
+         "decodes": 0, "prompts": 2, "chunk": 4001, "kv": 4001, "window": 0},
+        # a later chunk of a sliding layer of the released geometry, fp32 rows
+        {"name": "attn_sliding", "kind": "attn", "hd": 256, "n_kv": 16, "page": 32, "f16": False,
+         "decodes": 0, "prompts": 1, "chunk": 1111, "kv": 4114, "window": 1024},
+        # a prompt chunk beside 24 requests that decode
+        {"name": "attn_mixed", "kind": "attn", "hd": 128, "n_kv": 16, "page": 32, "f16": True,
+         "decodes": 24, "prompts": 1, "chunk": 500, "kv": 5000, "window": 0},
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choice(["plan", "append", "append", "attn", "attn", "attn"])
+    page = rng.choice([32, 64, 128])
+    if kind == "plan":
+        # from a few requests to a large batch, with and without finished ones
+        return {"kind": "plan", "seqs": _log(rng, 3, 1024), "page": page,
+                "width": _log(rng, 8, 256), "chunk": rng.choice([0, _log(rng, 5, 250)])}
+    hd, n_kv = rng.choice([(128, 16), (128, 8), (256, 16), (512, 4)])
+    f16 = rng.random() < 0.6
+    if kind == "append":
+        new = rng.choice([1, _log(rng, 2, 1500)])
+        seqs = _log(rng, 1, 96) if new == 1 else _log(rng, 1, max(1, 1500 // new))
+        return {"kind": "append", "hd": hd, "n_kv": n_kv, "page": page, "f16": f16,
+                "seqs": seqs, "new": new}
+    window = rng.choice([0, 0, 1024, _log(rng, 40, 2000)])
+    shape = rng.choice(["decode", "decode", "prompt", "mixed"])
+    if shape == "decode":
+        seqs = _log(rng, 1, 48)
+        return {"kind": "attn", "hd": hd, "n_kv": n_kv, "page": page, "f16": f16, "decodes": seqs,
+                "prompts": 0, "chunk": 0, "kv": _log(rng, 33, 160000 // seqs), "window": window}
+    prompts = rng.choice([1, 1, 2, 3])
+    chunk = _log(rng, 2, 1200 // prompts)
+    return {"kind": "attn", "hd": hd, "n_kv": n_kv, "page": page, "f16": f16,
+            "decodes": _log(rng, 1, 16) if shape == "mixed" else 0, "prompts": prompts,
+            "chunk": chunk, "kv": chunk + rng.choice([0, _log(rng, 1, 2000)]), "window": window}
+
+
+# ---- sizes that follow from a case alone -------------------------------------
+
+def _spread(n, lo, hi):
+    """n whole numbers of [lo, hi], spread evenly and in no order; the first is hi."""
+    return [hi - int((hi - lo) * ((i * 0.6180339887498949) % 1.0)) for i in range(n)]
+
+
+def _plan_lens(case):
+    """(cached, new, finished) of each row of a plan step."""
+    n, room = case["seqs"], case["width"] * case["page"]
+    chunk = min(case["chunk"], room)
+    ctx = _spread(n, 0, room - 1)
+    done = [1 if case["chunk"] and i % 8 == 3 else 0 for i in range(n)]
+    new = [chunk - i % min(chunk, 7) if d else 1 for i, d in enumerate(done)]
+    return ctx, new, done
+
+
+def _append_lens(case):
+    """(cached, new) of each request of an append step."""
+    page = case["page"]
+    return _spread(case["seqs"], 0, 5 * page - 3), [case["new"]] * case["seqs"]
+
+
+def _attn_lens(case):
+    """(cached and new, new) of each request: the decoding ones first."""
+    kv = _spread(case["decodes"], max(1, case["kv"] // 4), case["kv"])
+    new = [1] * case["decodes"]
+    kv += _spread(case["prompts"], max(case["chunk"], case["kv"] - case["kv"] // 4), case["kv"])
+    return kv, new + [case["chunk"]] * case["prompts"]
+
+
+def _pairs(case):
+    """Query-key pairs per query head, and the kv tokens that some query attends."""
+    pairs = toks = 0
+    for kv, new in zip(*_attn_lens(case)):
+        w = case["window"] or kv
+        first = kv - new
+        # position p attends min(p + 1, w) keys
+        ramp = max(0, min(kv, w) - first)  # queries that see fewer than w + 1 keys
+        pairs += sum(range(first + 1, first + ramp + 1)) + (new - ramp) * w
+        toks += kv - max(0, first + 1 - w)
+    return pairs, toks
+
+
+def _gathered(case):
+    """Tokens of the blocks that an append step writes to."""
+    ctx, new = _append_lens(case)
+    return sum(c + n - c // case["page"] * case["page"] for c, n in zip(ctx, new))
+
+
+def work(case):
+    if case["kind"] == "plan":
+        ctx, new, done = _plan_lens(case)
+        page = case["page"]
+        pages = sum(-(-((0 if d else c) + n) // page) - -(-(0 if d else c) // page)
+                    for c, n, d in zip(ctx, new, done))
+        given = sum(-(-c // page) for c, d in zip(ctx, done) if d)
+        return {"bytes": 4.0 * (4 * len(ctx) + sum(new) + 2 * pages + 3 * given), "flops": 0.0}
+    if case["kind"] == "append":
+        row = case["n_kv"] * case["hd"]
+        rows, back = sum(_append_lens(case)[1]), _gathered(case)
+        return {"bytes": 2.0 * row * (rows * ((2 if case["f16"] else 4) + 1) + back * (1 + 4)),
+                "flops": 0.0}
+    pairs, toks = _pairs(case)
+    rows = sum(_attn_lens(case)[1])
+    return {"bytes": 2.0 * toks * case["n_kv"] * case["hd"]
+            + 2.0 * rows * N_Q * case["hd"] * (2 if case["f16"] else 4),
+            "flops": 4.0 * pairs * N_Q * case["hd"]}
+
+
+# ---- inputs -------------------------------------------------------------------
+
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def _quants(gen, *shape):
+    """int8 quants of a normal distribution whose largest value is about 127."""
+    q = torch.randn(shape, generator=gen, device=DEV, dtype=torch.float16)
+    return q.mul_(36.0).round_().clamp_(-127, 127).to(torch.int8)
+
+
+def _scales(gen, *shape):
+    return 0.02 + 0.02 * torch.rand(shape, generator=gen, device=DEV)
+
+
+def _tables(lens, page, width, pages):
+    """Block tables of pages[0], pages[1], ... in request order; -1 behind each request."""
+    need = [-(-n // page) for n in lens]
+    t = torch.full((len(lens), width), -1, dtype=torch.int32)
+    at = 0
+    for i, n in enumerate(need):
+        t[i, :n] = pages[at:at + n]
+        at += n
+    return t.to(DEV), at
+
+
+def _cu(new):
+    return _i32([sum(new[:i]) for i in range(len(new) + 1)])
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device=DEV).manual_seed(seed * 9176 + 11)
+    host = torch.Generator().manual_seed(seed * 7919 + 5)
+    page = case["page"]
+    st = {"kind": case["kind"], "page": page}
+    if case["kind"] == "plan":
+        ctx, new, done = _plan_lens(case)
+        used = sum(-(-c // page) for c in ctx)
+        n_pages = used + sum(-(-n // page) + 1 for n in new) + 7
+        perm = torch.randperm(n_pages, generator=host).to(torch.int32)
+        tables, at = _tables(ctx, page, case["width"], perm)
+        free = torch.zeros(n_pages, dtype=torch.int32)
+        free[:n_pages - at] = perm[at:]
+        rows = -(-sum(new) // 64) * 64  # a graph's capacity: padded behind the last request
+        st |= {"ctx": _i32(ctx), "new": _i32(new), "done": _i32(done), "tables": tables,
+               "free": free.to(DEV), "n_free": _i32([n_pages - at]), "finish": any(done),
+               "lens": _i32(ctx), "tables_w": tables.clone(), "free_w": free.to(DEV),
+               "n_free_w": _i32([n_pages - at]), "n_free_out": _i32([0]),
+               "kv": _i32([0] * len(ctx)), "cu": _i32([0] * (len(ctx) + 1)),
+               "slots": _i32([-1] * rows), "missing": _i32([0])}
+        if own:
+            st["ctx_h"] = _context()
+        return st
+    hd, n_kv = case["hd"], case["n_kv"]
+    st |= {"hd": hd, "n_kv": n_kv}
+    typ = torch.float16 if case["f16"] else torch.float32
+    if case["kind"] == "append":
+        ctx, new = _append_lens(case)
+        first = [c // page * page for c in ctx]  # only the blocks from here on are touched
+        lens = [c + n - f for c, n, f in zip(ctx, new, first)]
+        n_pages = sum(-(-n // page) for n in lens) + 5
+        perm = torch.randperm(n_pages, generator=host).to(torch.int32)
+        tables, _ = _tables(lens, page, -(-max(lens) // page), perm)
+        tables = tables.cpu()
+
+        def slots(lo, hi):
+            pos = [(i, t) for i, (a, b) in enumerate(zip(lo, hi)) for t in range(a, b)]
+            s, t = (torch.tensor(v) for v in zip(*pos))
+            return (tables[s, t // page].long() * page + t % page).to(torch.int32).to(DEV)
+
+        off = [c - f for c, f in zip(ctx, first)]
+        rows = sum(new)
+        # K and V as the projections leave them: two slices of one row per token,
+        # with heads of different sizes
+        kv = torch.randn((rows, 2, n_kv, hd), generator=gen, device=DEV)
+        kv *= torch.exp(0.4 * torch.randn((1, 2, n_kv, 1), generator=gen, device=DEV))
+        kv = kv.to(typ)
+        st |= {"k": kv[:, 0], "v": kv[:, 1], "slots": slots(off, lens),
+               "back": slots([0] * len(lens), lens)}
+        m = st["back"].numel()
+        st |= {"k_out": torch.empty((m, n_kv, hd), device=DEV),
+               "v_out": torch.empty((m, n_kv, hd), device=DEV)}
+    else:
+        kv, new = _attn_lens(case)
+        need = sum(-(-n // page) for n in kv)
+        n_pages = need + need // 8 + 3
+        perm = torch.randperm(n_pages, generator=host).to(torch.int32)
+        width = -(-max(kv) // page) + 2
+        st["tables"], _ = _tables(kv, page, width, perm)
+        rows = sum(new)
+        st |= {"lens": _i32(kv), "cu": _cu(new), "max_new": max(new), "max_kv": max(kv),
+               "window": case["window"], "scale": 1.0 / math.sqrt(hd),
+               "q": torch.randn((rows, N_Q, hd), generator=gen, device=DEV).mul_(1.5).to(typ),
+               "out": torch.empty((rows, N_Q, hd), device=DEV, dtype=typ),
+               "scratch": torch.empty(64 << 20, dtype=torch.uint8, device=DEV)}
+    st |= {"kq": _quants(gen, n_pages, n_kv, page, hd),
+           "vq": _quants(gen, n_pages, n_kv, page // 32, hd, 32),
+           "ks": _scales(gen, n_pages, n_kv), "vs": _scales(gen, n_pages, n_kv)}
+    if own:
+        import sgq
+        st["ctx_h"] = _context()
+        st["pages"] = sgq.KvPages(st["kq"], st["vq"], st["ks"], st["vs"])
+    return st
+
+
+# ---- the framework's calls ------------------------------------------------------
+
+_ctx = None
+
+
+def _context():
+    """The program's context (one per process, on the current stream)."""
+    global _ctx
+    if _ctx is None:
+        at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                          "super-gemma_amd")
+        if at not in sys.path:
+            sys.path.insert(0, at)
+        import sgq
+        _ctx = sgq.GpuContext(0)
+    return _ctx
+
+
+def _run_own(st):
+    h = st["ctx_h"]
+    if st["kind"] == "plan":
+        lens, tables, free, n_free = st["ctx"], st["tables"], st["free"], st["n_free"]
+        if st["finish"]:  # on copies: a finished request's pages go back only once
+            lens, tables, free, n_free = st["lens"], st["tables_w"], st["free_w"], st["n_free_w"]
+            lens.copy_(st["ctx"])
+            tables.copy_(st["tables"])
+            free.copy_(st["free"])
+            n_free.copy_(st["n_free"])
+            h.kv_pages_release(st["done"], lens, tables, free, n_free, st["page"])
+        h.kv_pages_plan(lens, st["new"], tables, free, n_free, st["n_free_out"], st["kv"],
+                        st["cu"], st["slots"], st["missing"], st["page"])
+        return [tables, st["kv"], st["cu"], st["slots"], st["n_free_out"], st["missing"], free]
+    if st["kind"] == "append":
+        h.kv_append_paged_q8(st["pages"], st["k"], st["v"], st["slots"])
+        h.kv_gather_paged_q8(st["pages"], st["back"], st["k_out"], st["v_out"])
+        return [st["k_out"], st["v_out"], st["ks"], st["vs"]]
+    h.attn_paged_q8(st["pages"], st["q"], st["tables"], st["lens"], st["cu"], st["out"],
+                    max_new=st["max_new"], max_kv=st["max_kv"], window=st["window"],
+                    scale=st["scale"], workspace=st["scratch"])
+    return st["out"]
+
+
+# ---- the plain forms --------------------------------------------------------------
+
+def _plain_release(st):
+    lens, tables, page = st["ctx"].long(), st["tables"], st["page"]
+    done = st["done"] != 0
+    col = torch.arange(tables.shape[1], device=DEV)
+    held = done[:, None] & (col[None] < ((lens + page - 1) // page)[:, None]) & (tables >= 0)
+    given = tables[held]
+    free, n = st["free"].clone(), st["n_free"].long()
+    free[n + torch.arange(given.numel(), device=DEV)] = given
+    return (torch.where(done, 0, lens), torch.where(done[:, None], -1, tables), free,
+            n + given.numel())
+
+
+def _plain_plan(st):
+    page = st["page"]
+    lens, tables, free, n_free = _plain_release(st) if st["finish"] else (
+        st["ctx"].long(), st["tables"], st["free"], st["n_free"].long())
+    new = st["new"].long()
+    kv = lens + new
+    old_pages, all_pages = (lens + page - 1) // page, (kv + page - 1) // page
+    more = all_pages - old_pages
+    first = torch.cumsum(more, 0) - more  # pages taken by the requests before
+    col = torch.arange(tables.shape[1], device=DEV)
+    take = (col[None] >= old_pages[:, None]) & (col[None] < all_pages[:, None])
+    at = n_free - 1 - first[:, None] - (col[None] - old_pages[:, None])
+    tables = torch.where(take & (at >= 0), free[at.clamp(0, free.numel() - 1)],
+                         torch.where(take, -1, tables))
+    cu = torch.cat([new.new_zeros(1), torch.cumsum(new, 0)])
+    row = torch.arange(st["slots"].numel(), device=DEV)
+    s = (torch.searchsorted(cu, row, right=True) - 1).clamp(0, new.numel() - 1)
+    pos = lens[s] + row - cu[s]
+    p = tables[s, (pos // page).clamp(0, tables.shape[1] - 1)].long()
+    slots = torch.where((row < cu[-1]) & (p >= 0), p * page + pos % page, -1)
+    total = more.sum()
+    missing = ((slots < 0) & (row < cu[-1])).sum()
+    return [tables, kv.int(), cu.int(), slots.int(), (n_free - total).clamp(min=0).int(),
+            missing.int()[None], free]
+
+
+def _plain_write(quants, scales, x, slots, page):
+    """The pages [n_pages, n_kv, page, hd] after rows x went to their slots: a block
+    begun anew takes its scale from its new rows, another one's scale only grows
+    (and its quants are rounded to the grown one)."""
+    slots = slots.long()
+    at, off = slots // page, slots % page
+    most = x.abs().amax(-1)
+    amax = torch.zeros_like(scales).scatter_reduce_(0, at[:, None].expand_as(most), most, "amax")
+    need = (amax.double() / 127.0).float()
+    touched = torch.zeros(len(scales), dtype=torch.bool, device=DEV)
+    touched[at] = True
+    fresh = torch.zeros_like(touched)
+    fresh[at[off == 0]] = True
+    scale = torch.where(touched[:, None], torch.where(fresh[:, None], need,
+                                                      torch.maximum(scales, need)), scales)
+    grown = touched[:, None] & ~fresh[:, None] & (need > scales)
+    ratio = torch.where(grown, scales.double(), 0.0)[..., None, None]
+    grid = torch.where(grown, scale.double(), 1.0)[..., None, None]
+    quants = torch.where(grown[..., None, None], torch.round(quants.double() * ratio / grid),
+                         quants.double())
+    d = scale[at].double()[..., None]
+    quants[at, :, off] = torch.where(d > 0, torch.round(x.double() / torch.where(d > 0, d, 1.0)),
+                                     0.0)
+    return quants, scale
+
+
+def _rows_of_v(vq):
+    """V quants [n_pages, n_kv, page/32, hd, 32] as [n_pages, n_kv, page, hd]."""
+    return vq.transpose(-1, -2).flatten(2, 3)
+
+
+def _plain_append(st):
+    page, back = st["page"], st["back"].long()
+    at, off = back // page, back % page
+    kq, ks = _plain_write(st["kq"], st["ks"], st["k"].float(), st["slots"], page)
+    vq, vs = _plain_write(_rows_of_v(st["vq"]), st["vs"], st["v"].float(), st["slots"], page)
+    return [kq[at, :, off].float() * ks[at][..., None], vq[at, :, off].float() * vs[at][..., None],
+            ks, vs]
+
+
+def _plain_attn(st):
+    page, n_kv, hd = st["page"], st["n_kv"], st["hd"]
+    cu, lens, q = st["cu"].long(), st["lens"].long(), st["q"].float()
+    n = lens.numel()
+    # the requests' keys and values, padded to the longest
+    at = st["tables"][:, :-(-st["max_kv"] // page)].clamp(min=0).long()
+    k = st["kq"][at].float() * st["ks"][at][..., None, None]
+    v = _rows_of_v(st["vq"])[at.reshape(-1)].reshape(k.shape).float() * st["vs"][at][..., None, None]
+    k = k.permute(0, 2, 4, 1, 3).reshape(n * n_kv, hd, -1)
+    v = v.permute(0, 2, 1, 3, 4).reshape(n * n_kv, -1, hd)
+    # their query rows, padded to the longest chunk
+    i = torch.arange(st["max_new"], device=DEV)
+    new = cu[1:] - cu[:-1]
+    tok = (cu[:-1, None] + i).clamp(max=q.shape[0] - 1)
+    g = N_Q // n_kv
+    rows = q[tok].reshape(n, -1, n_kv, g, hd).permute(0, 2, 3, 1, 4).reshape(n * n_kv, -1, hd)
+    s = torch.bmm(rows, k).mul_(st["scale"]).view(n, n_kv, g, st["max_new"], -1)
+    pos = lens[:, None] - new[:, None] + i
+    key = torch.arange(s.shape[-1], device=DEV)
+    seen = key <= pos[..., None]
+    if st["window"]:
+        seen &= key > pos[..., None] - st["window"]
+    s.masked_fill_(~seen[:, None, None], -math.inf)
+    s -= s.amax(-1, keepdim=True)
+    s = s.exp_()
+    total = s.sum(-1, keepdim=True)
+    o = torch.bmm(s.view(n * n_kv, -1, s.shape[-1]), v).view(n, n_kv, g, -1, hd) / total
+    o = o.permute(0, 3, 1, 2, 4).reshape(n, -1, N_Q, hd)
+    out = torch.empty_like(st["out"])
+    live = i < new[:, None]
+    out[tok[live]] = o[live].to(out.dtype)
+    return out
+
+
+def run(st):
+    if own:
+        return _run_own(st)
+    if st["kind"] == "plan":
+        return _plain_plan(st)
+    if st["kind"] == "append":
+        return _plain_append(st)
+    return _plain_attn(st)
+
+
+# ---- the definitions in 64 bits ----------------------------------------------------
+
+def _exact_append(st):
+    page = st["page"]
+    slots = st["slots"].tolist()
+    pages = [s // page for s in slots]
+    # the runs of rows that go to one page
+    cuts = [i for i in range(len(slots)) if i == 0 or pages[i] != pages[i - 1]] + [len(slots)]
+    vals, scales = [], []
+    for x, q, d in ((st["k"], st["kq"], st["ks"]), (st["v"], _rows_of_v(st["vq"]), st["vs"])):
+        x, q, d = x.double(), q.double(), d.double()
+        for a, b in zip(cuts, cuts[1:]):
+            p = pages[a]
+            rows = torch.tensor([s % page for s in slots[a:b]], device=DEV)
+            most = x[a:b].abs().amax((0, 2)) / 127
+            most = most.float().double()  # the scale that is stored
+            if min(slots[a:b]) % page == 0:
+                d[p] = most
+            else:
+                up = torch.maximum(most, d[p])
+                if bool((up > d[p]).any()):
+                    was, now = d[p][:, None, None], up[:, None, None]
+                    q[p] = torch.where(now > was, (q[p] * was / now).round(), q[p])
+                d[p] = up
+            q[p][:, rows] = (x[a:b] / d[p][None, :, None]).round().nan_to_num(0.0).transpose(0, 1)
+        back = st["back"].long()
+        vals.append(q[back // page, :, back % page] * d[back // page][..., None])
+        scales.append(d)
+    return vals + scales
+
+
+def _exact_attn(st):
+    page, n_kv, hd = st["page"], st["n_kv"], st["hd"]
+    g = N_Q // n_kv
+    cu, lens, tables = st["cu"].tolist(), st["lens"].tolist(), st["tables"].long()
+    out = torch.zeros(st["out"].shape, dtype=torch.float64, device=DEV)
+    for b, kv in enumerate(lens):
+        a, e = cu[b], cu[b + 1]
+        j = torch.arange(kv, device=DEV)
+        p, o = tables[b, j // page], j % page
+        pos = torch.arange(kv - (e - a), kv, device=DEV)
+        seen = j[None] <= pos[:, None]
+        if st["window"]:
+            seen &= j[None] > pos[:, None] - st["window"]
+        for h in range(n_kv):
+            kh = st["kq"][p, h, o].double() * st["ks"][p, h].double()[:, None]
+            vh = st["vq"][p, h, o // 32, :, o % 32].double() * st["vs"][p, h].double()[:, None]
+            qh = st["q"][a:e, h * g:(h + 1) * g].double()
+            s = torch.tensordot(qh, kh.t().contiguous(), 1) * st["scale"]
+            s = torch.softmax(s.masked_fill(~seen[:, None], -math.inf), -1)
+            out[a:e, h * g:(h + 1) * g] = torch.tensordot(s, vh, 1)
+    return out
+
+
+def exact(case, seed):
+    if case["kind"] == "plan":
+        return None  # whole numbers only
+    st = prepare(case, seed)
+    return _exact_append(st) if case["kind"] == "append" else _exact_attn(st)
