@@ -345,6 +345,110 @@ int sgq_geglu(sgq_ctx *ctx, const float *gate, const float *up, float *y, uint64
 /* add_scaled.wgsl:21-27: y = (a + b)·s. */
 int sgq_add_scaled(sgq_ctx *ctx, const float *a, const float *b, float *y, uint64_t n, float s);
 
+/* ---- paged 8-bit KV cache of a batch of requests -------------------------- */
+/* No counterpart in the reference, which serves one request at a time: its
+ * caches are linear or rings, and so are those of the entry points above.
+ *
+ * The cache is a pool of pages.  A page holds page_size tokens (32, 64 or
+ * 128) of every kv head; slot = page * page_size + offset.  Each (page, head)
+ * is one block of int8 quants with one fp32 scale (finite, >= 0), for K and
+ * for V; a token's value is quant * scale:
+ *   k_quants [n_pages x n_kv_heads x page_size x head_dim]
+ *   v_quants [n_pages x n_kv_heads x page_size/32 x head_dim x 32]  (groups of
+ *            32 tokens transposed)
+ *   k_scales, v_scales [n_pages x n_kv_heads]
+ * head_dim 128, 256 or 512; 16-byte aligned quants.  A request's pages are
+ * the first entries of its row of block_tables [n_seqs x max_pages]; an entry
+ * outside 0..n_pages-1 stands for no page (its tokens are neither stored nor
+ * attended).  A page belongs to one request.
+ *
+ * A step is a packed batch: the new tokens of request 0, then of request 1,
+ * ..., one row each in q, k, v and out (act: SGQ_ACT_F32 or SGQ_ACT_F16 rows;
+ * strides between rows in elements, rows and strides 16-byte aligned).
+ * Everything is enqueued on the context's stream, allocates nothing, keeps
+ * nothing between calls and can be captured (sgq_graph_begin): lengths,
+ * tables and counters are read on the device.  Calls on different streams
+ * may overlap when they share no buffer that one of them writes. */
+typedef struct {
+    int8_t *k_quants;
+    int8_t *v_quants;
+    float *k_scales;
+    float *v_scales;
+    uint32_t n_pages, page_size, n_kv_heads, head_dim;
+} sgq_kv_pages;
+
+#define SGQ_ACT_F32 0
+#define SGQ_ACT_F16 1
+
+/* The tables of a step.  Request s has cached_lens[s] tokens in the cache and
+ * gets new_lens[s] more (negative lengths count as 0).  The pages it lacks are
+ * popped from the stack free_list [n_pages], of which *n_free entries are in
+ * use, in request order (the i-th is free_list[*n_free - 1 - i]) and written
+ * to its table row; where the stack runs out, -1.  Also written:
+ *   kv_lens [n_seqs]        cached + new
+ *   cu_tokens [n_seqs + 1]  the first packed row of each request, and the end
+ *   slot_map [n_tokens]     each packed row's slot, -1 behind the last request
+ *                           and for tokens without a page (table row or pool
+ *                           exhausted)
+ *   missing [1]             how many tokens got no slot, or no row in slot_map
+ *   n_free_out [1]          the entries left
+ * kv_lens may be cached_lens and n_free_out may be n_free (a captured step
+ * that advances itself).  n_seqs <= 4096. */
+int sgq_kv_pages_plan(sgq_ctx *ctx, const int32_t *cached_lens, const int32_t *new_lens,
+                      uint32_t n_seqs, uint32_t page_size, int32_t *block_tables,
+                      uint32_t max_pages, const int32_t *free_list, uint32_t n_pages,
+                      const int32_t *n_free, int32_t *n_free_out, int32_t *kv_lens,
+                      int32_t *cu_tokens, int32_t *slot_map, uint32_t n_tokens, int32_t *missing);
+/* Gives back the pages of the requests with done[s] != 0: the
+ * ceil(kv_lens[s] / page_size) first entries of their table rows are pushed on
+ * free_list, in request and table order (entries that stand for no page are
+ * left out), their table rows become -1 and their kv_lens 0. */
+int sgq_kv_pages_release(sgq_ctx *ctx, const int32_t *done, uint32_t n_seqs, uint32_t page_size,
+                         int32_t *kv_lens, int32_t *block_tables, uint32_t max_pages,
+                         int32_t *free_list, uint32_t n_pages, int32_t *n_free);
+/* Writes the rows k and v [n_tokens x n_kv_heads x head_dim] to their slots
+ * (rows with a slot outside the cache are skipped).  Consecutive rows of one
+ * page are one run; with d = max|x| / 127 over a head's part of the run, a run
+ * that holds the page's first slot begins the block anew with scale d (what
+ * the page held is gone), any other leaves scale max(old, d), the block's
+ * quants rounded to the scale when it grew.  quants = x / scale, to nearest,
+ * ties to even.  An infinity or NaN in a row makes its block's scale NaN.
+ * A slot named twice in a run takes the later row.  The rows of one page must
+ * be consecutive in slot_map: two runs of one page in one call leave that
+ * page's contents unspecified. */
+int sgq_kv_append_paged_q8(sgq_ctx *ctx, const sgq_kv_pages *pages, const void *k,
+                           uint64_t k_stride, const void *v, uint64_t v_stride, int act,
+                           const int32_t *slot_map, uint32_t n_tokens);
+/* The values of slots: rows k and v [n_tokens x n_kv_heads x head_dim] =
+ * quant * scale (f16: rounded once).  Rows with a slot outside the cache are
+ * left as they were. */
+int sgq_kv_gather_paged_q8(sgq_ctx *ctx, const sgq_kv_pages *pages, const int32_t *slot_map,
+                           uint32_t n_tokens, int act, void *k, uint64_t k_stride, void *v,
+                           uint64_t v_stride);
+/* Attention of a step's rows q [n_tokens x n_q_heads x head_dim] over the
+ * pages (after the step's append): request s has the rows
+ * cu_tokens[s]..cu_tokens[s+1]-1, its last ones at position kv_lens[s]-1; a
+ * row at position p attends positions <= p, with window > 0 only those
+ * > p - window, and query head h reads kv head h / (n_q_heads/n_kv_heads).
+ * out [n_tokens x n_q_heads x head_dim] of q's type; a row that attends
+ * nothing is 0, rows behind the last request are left as they were.
+ * max_new: no request has more rows than this (rows past it are not
+ * computed).  max_kv: about the longest kv_lens, by which the keys of long
+ * requests are split over workgroups; any value gives the same result up to
+ * rounding.  workspace: device memory for those splits, not shared by calls
+ * (or graphs) that may overlap; sgq_attn_paged_workspace says how much is
+ * used, with less (or NULL) the keys are split less.
+ * fp32 rows are computed to fp32 accuracy (22-bit q and weights, fp32 sums);
+ * f16 rows with f16 weights. */
+uint64_t sgq_attn_paged_workspace(const sgq_kv_pages *pages, uint32_t n_seqs, uint32_t n_tokens,
+                                  uint32_t n_q_heads, uint32_t max_new, uint32_t max_kv);
+int sgq_attn_paged_q8(sgq_ctx *ctx, const sgq_kv_pages *pages, const void *q, uint64_t q_stride,
+                      int act, const int32_t *block_tables, uint32_t max_pages,
+                      const int32_t *kv_lens, const int32_t *cu_tokens, uint32_t n_seqs,
+                      uint32_t n_tokens, uint32_t n_q_heads, uint32_t max_new, uint32_t max_kv,
+                      uint32_t window, float scale, void *out, uint64_t out_stride,
+                      void *workspace, uint64_t workspace_bytes);
+
 /* ---- decode-step driver ------------------------------------------------- */
 /* A random-init decoder of the reference's model family (the CPU forward pass
  * crates/sg-model/src/reference.rs:157-316 and the GPU graph

@@ -14,7 +14,7 @@
 #include <string>
 #include <vector>
 
-#include "sgq_internal.h"
+#include "paged.h"
 
 struct sgq_ctx {
     int device = 0;
@@ -63,6 +63,7 @@ const DeviceInfo &device_info() {
 
 hipStream_t ctx_stream(const sgq_ctx *ctx) { return ctx ? ctx->stream : nullptr; }
 void *ctx_workspace(const sgq_ctx *ctx) { return ctx ? ctx->workspace : nullptr; }
+int ctx_device(const sgq_ctx *ctx) { return ctx ? ctx->device : 0; }
 
 }  // namespace sgq
 

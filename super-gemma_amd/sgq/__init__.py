@@ -90,6 +90,12 @@ class ModelConfig(C.Structure):
         return {n: getattr(self, n) for n, _ in self._fields_}
 
 
+class _KvPages(C.Structure):
+    """sgq_kv_pages (include/sgq.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("k_quants", "v_quants", "k_scales", "v_scales")] + [
+        (n, C.c_uint32) for n in ("n_pages", "page_size", "n_kv_heads", "head_dim")]
+
+
 class _GgufTensor(C.Structure):
     _fields_ = [("name", C.c_char_p), ("type", C.c_uint32), ("n_dims", C.c_uint32),
                 ("dims", C.c_uint64 * 4), ("offset", C.c_uint64), ("bytes", C.c_uint64),
@@ -161,6 +167,13 @@ SIGNATURES = {
     "sgq_gguf_meta_float": (I, [P, C.c_char_p, C.POINTER(C.c_double)]),
     "sgq_gguf_meta_string": (I, [P, C.c_char_p, C.POINTER(C.c_char_p)]),
     "sgq_model_load_gguf": (I, [P, P]),
+    "sgq_kv_pages_plan": (I, [P, P, P, U32, U32, P, U32, P, U32, P, P, P, P, P, U32, P]),
+    "sgq_kv_pages_release": (I, [P, P, U32, U32, P, P, U32, P, U32, P]),
+    "sgq_kv_append_paged_q8": (I, [P, P, P, U64, P, U64, I, P, U32]),
+    "sgq_kv_gather_paged_q8": (I, [P, P, P, U32, I, P, U64, P, U64]),
+    "sgq_attn_paged_workspace": (U64, [P, U32, U32, U32, U32, U32]),
+    "sgq_attn_paged_q8": (I, [P, P, P, U64, I, P, U32, P, P, U32, U32, U32, U32, U32, U32,
+                              C.c_float, P, U64, P, U64]),
     "sgq_fill_q4_0_random": (I, [P, P, U64, U64, C.c_float]),
     "sgq_fill_normal": (I, [P, P, U64, U64, C.c_float, C.c_float]),
 }
@@ -236,6 +249,70 @@ class StepState:
     kv_len_sliding: int = 0
     kv_len_global: int = 0
     q0: int = 0
+
+
+class KvPages:
+    """The pool of a paged 8-bit KV cache (sgq_kv_pages, include/sgq.h) over
+    torch tensors: k_quants int8 [n_pages, n_kv, page_size, head_dim], v_quants
+    int8 [n_pages, n_kv, page_size/32, head_dim, 32], scales fp32
+    [n_pages, n_kv].  Checked once here; keep it as long as the cache."""
+
+    def __init__(self, k_quants: torch.Tensor, v_quants: torch.Tensor, k_scales: torch.Tensor,
+                 v_scales: torch.Tensor):
+        if k_quants.dim() != 4:
+            raise ValidationError(6, "k_quants: [n_pages, n_kv, page_size, head_dim] expected")
+        n, h, p, d = k_quants.shape
+        if tuple(v_quants.shape) != (n, h, p // 32, d, 32) or p % 32:
+            raise ValidationError(6, "v_quants: [n_pages, n_kv, page_size/32, head_dim, 32] expected")
+        if tuple(k_scales.shape) != (n, h) or tuple(v_scales.shape) != (n, h):
+            raise ValidationError(6, "scales: [n_pages, n_kv] expected")
+        _need(k_quants, torch.int8, 1, "k_quants")
+        _need(v_quants, torch.int8, 1, "v_quants")
+        _need(k_scales, torch.float32, 1, "k_scales")
+        _need(v_scales, torch.float32, 1, "v_scales")
+        self.tensors = (k_quants, v_quants, k_scales, v_scales)
+        if len({t.device for t in self.tensors}) != 1:
+            raise ValidationError(6, "pages on different devices")
+        self.device = k_quants.device
+        self.n_pages, self.n_kv, self.page_size, self.head_dim = n, h, p, d
+        self._s = _KvPages(*(_ptr(t) for t in self.tensors), n, p, h, d)
+        self._p = C.addressof(self._s)
+
+    @staticmethod
+    def empty(n_pages: int, page_size: int, n_kv: int, head_dim: int, device="cuda") -> "KvPages":
+        """A pool of zeroed pages."""
+        def z(shape, t):
+            return torch.zeros(shape, dtype=t, device=device)
+        return KvPages(z((n_pages, n_kv, page_size, head_dim), torch.int8),
+                       z((n_pages, n_kv, page_size // 32, head_dim, 32), torch.int8),
+                       z((n_pages, n_kv), torch.float32), z((n_pages, n_kv), torch.float32))
+
+
+_ACT = {torch.float32: 0, torch.float16: 1}
+
+
+def _i32(t, n, dev, name):
+    """Device pointer of an int32 tensor of at least n elements."""
+    if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous() or t.numel() < n:
+        raise ValidationError(6, f"{name}: contiguous int32 tensor of {n} elements on {dev} expected, "
+                                 f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _rows(t, heads, hd, dev, name):
+    """(device pointer, row stride) of packed rows [n, heads, hd] (fp32 or f16),
+    whose rows may lie apart."""
+    if (t.dtype not in _ACT or t.device != dev or t.dim() != 3 or t.shape[1] != heads or
+            t.shape[2] != hd or t.stride(2) != 1 or t.stride(1) != hd):
+        raise ValidationError(6, f"{name}: fp32 or f16 rows [n, {heads}, {hd}] on {dev} expected, "
+                                 f"got {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
+    stride = t.stride(0)
+    if t.shape[0] < 2:
+        stride = max(stride, heads * hd)  # no second row to reach
+        stride += -stride % 8
+    if stride < heads * hd:
+        raise ValidationError(6, f"{name}: rows overlap (stride {stride})")
+    return t.data_ptr(), stride
 
 
 class GpuContext:
@@ -443,6 +520,91 @@ class GpuContext:
         _need(a, torch.float32, n, "a")
         _need(b, torch.float32, n, "b")
         _check(lib().sgq_add_scaled(self._h, _ptr(a), _ptr(b), _ptr(y), n, s))
+
+    # -- paged 8-bit KV cache of a batch of requests --------------------------
+    def _dev(self):
+        return torch.device("cuda", self.device)
+
+    def kv_pages_plan(self, cached_lens, new_lens, block_tables, free_list, n_free, n_free_out,
+                      kv_lens, cu_tokens, slot_map, missing, page_size: int):
+        """Block tables, row offsets and slot map of a step from the requests'
+        lengths (sgq_kv_pages_plan).  block_tables [n_seqs, max_pages]; all int32."""
+        dev, n = self._dev(), cached_lens.numel()
+        if block_tables.dim() != 2 or block_tables.shape[0] != n:
+            raise ValidationError(6, f"block_tables: [{n}, max_pages] expected")
+        _check(lib().sgq_kv_pages_plan(
+            self._h, _i32(cached_lens, n, dev, "cached_lens"), _i32(new_lens, n, dev, "new_lens"), n,
+            page_size, _i32(block_tables, n, dev, "block_tables"), block_tables.shape[1],
+            _i32(free_list, 1, dev, "free_list"), free_list.numel(), _i32(n_free, 1, dev, "n_free"),
+            _i32(n_free_out, 1, dev, "n_free_out"), _i32(kv_lens, n, dev, "kv_lens"),
+            _i32(cu_tokens, n + 1, dev, "cu_tokens"), _i32(slot_map, 0, dev, "slot_map"),
+            slot_map.numel(), _i32(missing, 1, dev, "missing")))
+
+    def kv_pages_release(self, done, kv_lens, block_tables, free_list, n_free, page_size: int):
+        """Give back the pages of the requests with done != 0 (sgq_kv_pages_release)."""
+        dev, n = self._dev(), kv_lens.numel()
+        if block_tables.dim() != 2 or block_tables.shape[0] != n:
+            raise ValidationError(6, f"block_tables: [{n}, max_pages] expected")
+        _check(lib().sgq_kv_pages_release(
+            self._h, _i32(done, n, dev, "done"), n, page_size, _i32(kv_lens, n, dev, "kv_lens"),
+            _i32(block_tables, n, dev, "block_tables"), block_tables.shape[1],
+            _i32(free_list, 1, dev, "free_list"), free_list.numel(), _i32(n_free, 1, dev, "n_free")))
+
+    def _kv_rows(self, pages: KvPages, k, v, slot_map):
+        dev = self._dev()
+        if pages.device != dev:
+            raise ValidationError(6, f"pages on {pages.device}, context on {dev}")
+        kp, ks = _rows(k, pages.n_kv, pages.head_dim, dev, "k")
+        vp, vs = _rows(v, pages.n_kv, pages.head_dim, dev, "v")
+        n = slot_map.numel()
+        if k.dtype != v.dtype or k.shape[0] < n or v.shape[0] < n:
+            raise ValidationError(6, f"k, v: {n} rows of one type expected")
+        return kp, ks, vp, vs, _i32(slot_map, n, dev, "slot_map"), n, _ACT[k.dtype]
+
+    def kv_append_paged_q8(self, pages: KvPages, k, v, slot_map):
+        """Write the rows k, v [n, n_kv, head_dim] to their slots (sgq_kv_append_paged_q8)."""
+        kp, ks, vp, vs, sp, n, act = self._kv_rows(pages, k, v, slot_map)
+        _check(lib().sgq_kv_append_paged_q8(self._h, pages._p, kp, ks, vp, vs, act, sp, n))
+
+    def kv_gather_paged_q8(self, pages: KvPages, slot_map, k, v):
+        """The values of slots into rows k, v [n, n_kv, head_dim] (sgq_kv_gather_paged_q8)."""
+        kp, ks, vp, vs, sp, n, act = self._kv_rows(pages, k, v, slot_map)
+        _check(lib().sgq_kv_gather_paged_q8(self._h, pages._p, sp, n, act, kp, ks, vp, vs))
+
+    def attn_paged_workspace(self, pages: KvPages, n_seqs: int, n_tokens: int, n_q: int,
+                             max_new: int, max_kv: int) -> int:
+        """Bytes of workspace with which attn_paged_q8 splits long requests freely."""
+        return int(lib().sgq_attn_paged_workspace(pages._p, n_seqs, n_tokens, n_q, max_new, max_kv))
+
+    def attn_paged_q8(self, pages: KvPages, q, block_tables, kv_lens, cu_tokens, out, max_new: int,
+                      max_kv: Optional[int] = None, window: int = 0,
+                      scale: Optional[float] = None, workspace: Optional[torch.Tensor] = None):
+        """Attention of the packed rows q [n, n_q, head_dim] over the pages
+        (sgq_attn_paged_q8): request s has rows cu_tokens[s]..cu_tokens[s+1]-1, the
+        last at position kv_lens[s]-1.  max_kv: about the longest kv_lens (None:
+        what the tables hold)."""
+        dev, n = self._dev(), kv_lens.numel()
+        if pages.device != dev:
+            raise ValidationError(6, f"pages on {pages.device}, context on {dev}")
+        if block_tables.dim() != 2 or block_tables.shape[0] != n:
+            raise ValidationError(6, f"block_tables: [{n}, max_pages] expected")
+        hd, width = pages.head_dim, block_tables.shape[1]
+        n_q = q.shape[1] if q.dim() == 3 else 0
+        qp, qs = _rows(q, n_q, hd, dev, "q")
+        op, os_ = _rows(out, n_q, hd, dev, "out")
+        rows = q.shape[0]
+        if out.dtype != q.dtype or out.shape[0] < rows:
+            raise ValidationError(6, f"out: {rows} rows of {q.dtype} expected")
+        wp, wb = None, 0
+        if workspace is not None:
+            if workspace.device != dev or not workspace.is_contiguous():
+                raise ValidationError(6, f"workspace: contiguous tensor on {dev} expected")
+            wp, wb = workspace.data_ptr(), _nbytes(workspace)
+        _check(lib().sgq_attn_paged_q8(
+            self._h, pages._p, qp, qs, _ACT[q.dtype], _i32(block_tables, n, dev, "block_tables"), width,
+            _i32(kv_lens, n, dev, "kv_lens"), _i32(cu_tokens, n + 1, dev, "cu_tokens"), n, rows, n_q,
+            max_new, width * pages.page_size if max_kv is None else max_kv, window,
+            hd ** -0.5 if scale is None else scale, op, os_, wp, wb))
 
     def fill_q4_0_random(self, w: torch.Tensor, n_blocks: int, seed: int, sigma: float = 0.02):
         _need(w, torch.uint8, n_blocks * 18, "w")
