@@ -272,8 +272,8 @@ def prepare(case, seed):
            "vq": _quants(gen, n_pages, n_kv, page // 32, hd, 32),
            "ks": _scales(gen, n_pages, n_kv), "vs": _scales(gen, n_pages, n_kv)}
     if own:
-        import sgq
         st["ctx_h"] = _context()
+        import sgq
         st["pages"] = sgq.KvPages(st["kq"], st["vq"], st["ks"], st["vs"])
     return st
 
