@@ -381,7 +381,8 @@ typedef struct {
 #define SGQ_ACT_F16 1
 
 /* The tables of a step.  Request s has cached_lens[s] tokens in the cache and
- * gets new_lens[s] more (negative lengths count as 0).  The pages it lacks are
+ * gets new_lens[s] more (negative lengths count as 0, new ones above 2^22, the
+ * most rows of a step, as 2^22).  The pages it lacks are
  * popped from the stack free_list [n_pages], of which *n_free entries are in
  * use, in request order (the i-th is free_list[*n_free - 1 - i]) and written
  * to its table row; where the stack runs out, -1.  Also written:

@@ -8,15 +8,17 @@
 // position c_s + i, whose slot is table[s][pos/P]·P + pos%P.
 //
 // A few kilobytes: what counts is the launch and the chain of dependent
-// loads.  One workgroup scans both sums in LDS and fills everything: the
-// thread of a row (or of a popped page) finds its request by bisection in the
-// LDS sums.
+// loads.  One workgroup scans both sums in LDS and pops the pages: the thread of
+// a page (or of a row) finds its request by bisection in the LDS sums.  It fills
+// the slot map too while that is one or two rows a thread (kPlanRows); a longer
+// one goes to a second launch over the whole GPU.
 #include "paged.h"
 
 namespace sgq {
 namespace {
 
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanRows = 2 * kPlanThreads;
 
 // Inclusive sums over the workgroup of one value a thread.
 template <int NT>
@@ -55,6 +57,30 @@ __device__ __forceinline__ int clamp_len(long long v) {
     return v < 0 ? 0 : v > 0x7fffffff ? 0x7fffffff : (int)v;
 }
 
+__device__ __forceinline__ int clamp_new(int n) { return min(max(n, 0), 1 << 22); }
+
+// Rows first, first + step, ... of the slot map; how many of them got no slot.
+template <typename Cached>
+__device__ __forceinline__ int fill_rows(const PagedPlan &p, const int *cu_s, int n_rows, int first,
+                                         int step, Cached cached) {
+    int lost = 0;
+    for (int r = first; r < p.n_tokens; r += step) {
+        int slot = -1;
+        if (r < n_rows) {
+            const int s = find_owner(cu_s, p.n_seqs, r);
+            const long long pos = (long long)cached(s) + (r - cu_s[s]);
+            const long long e = pos >> p.page_log2;
+            const int page = e < p.max_pages ? p.tables[(size_t)s * p.max_pages + e] : -1;
+            if ((unsigned)page < (unsigned)p.n_pages)
+                slot = (page << p.page_log2) + (int)(pos & ((1 << p.page_log2) - 1));
+            else
+                lost++;
+        }
+        p.slots[r] = slot;
+    }
+    return lost;
+}
+
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlan p) {
     __shared__ int cu_s[kPagedMaxSeqs + 1];
     __shared__ int pg_s[kPagedMaxSeqs + 1];
@@ -70,7 +96,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlan p) {
         int c = 0, n = 0, more = 0;
         if (s < p.n_seqs) {
             c = max(p.cached[s], 0);
-            n = max(p.add[s], 0);
+            n = min(clamp_new(p.add[s]), 0x7fffffff - c);  // c + n and, up to 2^22 rows, cu are exact
             const long long cap = (long long)p.max_pages;
             long long have = ((long long)c + P - 1) >> p.page_log2;
             long long want = ((long long)c + n + P - 1) >> p.page_log2;
@@ -106,28 +132,30 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlan p) {
         p.tables[(size_t)s * p.max_pages + have + (i - pg_s[s])] = at >= 0 ? p.free_list[at] : -1;
     }
     __syncthreads();
-    // the rows
-    int lost = 0;
-    for (int r = tid; r < p.n_tokens; r += kPlanThreads) {
-        int slot = -1;
-        if (r < n_rows) {
-            const int s = find_owner(cu_s, p.n_seqs, r);
-            const long long pos = (long long)cached_s[s] + (r - cu_s[s]);
-            const long long e = pos >> p.page_log2;
-            const int page = e < p.max_pages ? p.tables[(size_t)s * p.max_pages + e] : -1;
-            if ((unsigned)page < (unsigned)p.n_pages)
-                slot = (page << p.page_log2) + (int)(pos & (P - 1));
-            else
-                lost++;
-        }
-        p.slots[r] = slot;
+    if (tid == 0) *p.n_free_out = max(n_free - n_new, 0);
+    const int over = max(n_rows - p.n_tokens, 0);  // rows that the map does not hold
+    if (p.n_tokens > kPlanRows) {
+        if (tid == 0) *p.missing = over;  // the next launch adds to it
+        return;
     }
+    const int lost = fill_rows(p, cu_s, n_rows, tid, kPlanThreads, [&](int s) { return cached_s[s]; });
     if (lost) atomicAdd(&missing_s, lost);
     __syncthreads();
-    if (tid == 0) {
-        *p.missing = missing_s + max(n_rows - p.n_tokens, 0);
-        *p.n_free_out = max(n_free - n_new, 0);
-    }
+    if (tid == 0) *p.missing = missing_s + over;
+}
+
+// The slot map of many rows; kv_lens and cu are the scan's.
+constexpr int kRowsThreads = 256;
+__global__ __launch_bounds__(kRowsThreads) void paged_plan_rows_kernel(PagedPlan p) {
+    __shared__ int cu_s[kPagedMaxSeqs + 1];
+    for (int s = threadIdx.x; s <= p.n_seqs; s += kRowsThreads) cu_s[s] = p.cu[s];
+    __syncthreads();
+    int lost = fill_rows(p, cu_s, cu_s[p.n_seqs], blockIdx.x * kRowsThreads + threadIdx.x,
+                         gridDim.x * kRowsThreads,
+                         [&](int s) { return p.kv_lens[s] - (cu_s[s + 1] - cu_s[s]); });
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) lost += __shfl_xor(lost, d);
+    if (lost && (threadIdx.x & 63) == 0) atomicAdd(p.missing, lost);  // whole numbers: any order
 }
 
 // Pages go back in request order, a request's pages in table order.
@@ -152,29 +180,61 @@ __global__ __launch_bounds__(kPlanThreads) void paged_release_kernel(PagedReleas
     const int n_held = clamp_len(pg0);
     if (tid == 0) pg_s[p.n_seqs] = n_held;
     __syncthreads();
-    // entries outside the pool are dropped: the pushed ones are counted in order
+    // entries outside the pool are dropped: the pushed ones are counted in order,
+    // 8 rounds of a thread per page at a time
+    constexpr int kRounds = 8, kWaves = kPlanThreads / 64;
+    __shared__ int count_s[kRounds * kWaves];
+    const int lane = tid & 63, wave = tid >> 6;
     int top = n_free;
-    for (int b = 0; b < n_held; b += kPlanThreads) {
-        const int i = b + tid;
-        int page = -1;
-        if (i < n_held) {
-            const int s = find_owner(pg_s, p.n_seqs, i);
-            page = p.tables[(size_t)s * p.max_pages + (i - pg_s[s])];
+    for (int b = 0; b < n_held; b += kRounds * kPlanThreads) {
+        int page[kRounds];
+        uint64_t in[kRounds];
+#pragma unroll
+        for (int k = 0; k < kRounds; k++) {
+            const int i = b + k * kPlanThreads + tid;
+            page[k] = -1;
+            if (i >= 0 && i < n_held) {
+                const int s = find_owner(pg_s, p.n_seqs, i);
+                page[k] = p.tables[(size_t)s * p.max_pages + (i - pg_s[s])];
+            }
         }
-        const bool ok = (unsigned)page < (unsigned)p.n_pages;
-        long long all;
-        const long long at = top + block_scan<kPlanThreads>(ok, wave_s, &all) - 1;
-        if (ok && at < p.n_pages) p.free_list[at] = page;
-        top = (int)min((long long)p.n_pages, top + all);
+#pragma unroll
+        for (int k = 0; k < kRounds; k++) in[k] = __ballot((unsigned)page[k] < (unsigned)p.n_pages);
+        __syncthreads();  // count_s of the last rounds has been read
+        if (lane < kRounds) {
+            uint64_t mine = in[0];
+#pragma unroll
+            for (int k = 1; k < kRounds; k++) mine = lane == k ? in[k] : mine;
+            count_s[lane * kWaves + wave] = __popcll(mine);
+        }
+        __syncthreads();
+        int at = top;
+#pragma unroll
+        for (int k = 0; k < kRounds; k++) {
+            int before = 0, all = 0;
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) {
+                const int c = count_s[k * kWaves + w];
+                before += w < wave ? c : 0;
+                all += c;
+            }
+            const int to = at + before + __popcll(in[k] & ((1ull << lane) - 1));
+            if (in[k] >> lane & 1 && to < p.n_pages) p.free_list[to] = page[k];
+            at += all;
+        }
+        top = min(at, p.n_pages);
     }
     __syncthreads();
-    for (int s = 0; s < p.n_seqs; s++) {
-        if (!p.done[s]) continue;
-        for (int j = tid; j < p.max_pages; j += kPlanThreads)
-            p.tables[(size_t)s * p.max_pages + j] = -1;
+    // a wave clears the rows of 64 requests: only finished ones cost a store
+    for (int b = (tid >> 6) * 64; b < p.n_seqs; b += kPlanThreads) {
+        const int s = b + (tid & 63);
+        const bool done = s < p.n_seqs && p.done[s];
+        if (done) p.kv_lens[s] = 0;
+        for (uint64_t m = __ballot(done); m; m &= m - 1) {
+            int32_t *row = p.tables + (size_t)(b + __builtin_ctzll(m)) * p.max_pages;
+            for (int j = tid & 63; j < p.max_pages; j += 64) row[j] = -1;
+        }
     }
-    for (int s = tid; s < p.n_seqs; s += kPlanThreads)
-        if (p.done[s]) p.kv_lens[s] = 0;
     if (tid == 0) *p.n_free = top;
 }
 
@@ -183,6 +243,12 @@ __global__ __launch_bounds__(kPlanThreads) void paged_release_kernel(PagedReleas
 int launch_paged_plan(hipStream_t st, const PagedPlan &p) {
     hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p);
     SGQ_HIP(hipGetLastError());
+    if (p.n_tokens > kPlanRows) {
+        const int wgs = (p.n_tokens + kRowsThreads - 1) / kRowsThreads;
+        hipLaunchKernelGGL(paged_plan_rows_kernel, dim3(wgs < 512 ? wgs : 512), dim3(kRowsThreads), 0,
+                           st, p);
+        SGQ_HIP(hipGetLastError());
+    }
     return SGQ_OK;
 }
 
