@@ -103,6 +103,14 @@ __device__ __forceinline__ int key_hi(const AttnArgs &a, int pos, int kv_len) {
     return clamped(min(pos + 1, kv_len), 0, cap);
 }
 
+// The positions of a row tile's first and last row.
+__device__ __forceinline__ int first_pos(const AttnArgs &a, const RowTile &rt) {
+    return rt.kv_len - rt.new_len + rt.row0 / a.group;
+}
+__device__ __forceinline__ int last_pos(const AttnArgs &a, const RowTile &rt) {
+    return rt.kv_len - rt.new_len + (rt.row0 + rt.rows - 1) / a.group;
+}
+
 // Which 32-key tiles a row tile attends, and into how many parts of `per`
 // tiles they are cut: parts of one length for all requests, so that a long one
 // has more of them, unless that makes more than `splits`.
@@ -110,11 +118,9 @@ struct KeySpan {
     int t0, t1, parts, per;
 };
 __device__ __forceinline__ KeySpan key_span(const AttnArgs &a, const RowTile &rt, int splits, int per) {
-    const int first = rt.kv_len - rt.new_len + rt.row0 / a.group;
-    const int last = rt.kv_len - rt.new_len + (rt.row0 + rt.rows - 1) / a.group;
     KeySpan k;
-    k.t0 = key_lo(a, first) >> 5;
-    k.t1 = max((key_hi(a, last, rt.kv_len) + 31) >> 5, k.t0);
+    k.t0 = key_lo(a, first_pos(a, rt)) >> 5;
+    k.t1 = max((key_hi(a, last_pos(a, rt), rt.kv_len) + 31) >> 5, k.t0);
     const int n = k.t1 - k.t0;
     k.per = max(per, (n + splits - 1) / splits);
     k.parts = max((n + k.per - 1) / k.per, 1);
@@ -159,6 +165,29 @@ __device__ __forceinline__ V load(const int8_t *p) {
     return STREAM ? __builtin_nontemporal_load(v) : *v;
 }
 
+// The pages of 64 tiles and what their scales make of the scores: one tile a lane,
+// read lane by lane.
+struct TilePages {
+    int page;            // 0 where there is none
+    float ks, lv, rv;    // K scale; log2 and reciprocal of the V scale
+    // Lane i: tile t + i·step, if that is below t1.
+    __device__ __forceinline__ void load(const AttnArgs &a, const int32_t *table, int head, int t, int step, int t1) {
+        const int mine = t + (threadIdx.x & 63) * step;
+        const int p = mine < t1 ? table[mine >> (a.pg.page_log2 - 5)] : -1;
+        const bool ok = (unsigned)p < (unsigned)a.pg.n_pages;
+        page = ok ? p : 0;
+        const size_t b = (size_t)page * a.pg.n_kv + head;
+        const float raw = a.pg.vs[b];
+        const float vs = fmaxf(raw, kMinScale) + (raw - raw);  // NaN stays
+        ks = ok ? a.pg.ks[b] : 0.f;
+        lv = ok ? __builtin_amdgcn_logf(vs) : -INFINITY;  // no page: no weight
+        rv = ok && vs == vs ? 1.f / vs : 1.f;             // finite: a masked key's 0·rv stays 0
+    }
+    __device__ __forceinline__ void scales(int lane, float (&sc)[3]) const {
+        sc[0] = lane_f(ks, lane), sc[1] = lane_f(lv, lane), sc[2] = lane_f(rv, lane);
+    }
+};
+
 __device__ __forceinline__ float fmax16(float v) {  // over the lanes of a column
     v = fmaxf(v, __shfl_xor(v, 16));
     return fmaxf(v, __shfl_xor(v, 32));
@@ -184,6 +213,8 @@ struct Wave {
     f4 acc[NT][ND];
     float M[NT], l[NT];
 
+    // RAISED: K will come as quants_f16_raised.
+    template <bool RAISED>
     __device__ __forceinline__ void load_q(const AttnArgs &a, const RowTile &rt, int head, int n, int g) {
 #pragma unroll
         for (int i = 0; i < NT; i++) {
@@ -233,11 +264,103 @@ struct Wave {
 #pragma unroll
                         for (int j = 0; j < 8; j++) sum += (float)qa[i][c][h][j];
                     }
-                sum += __shfl_xor(sum, 16);
-                sum += __shfl_xor(sum, 32);
-                row_raise[i] = -128.f * sum * row_scale[i];
-                row_scale[i] *= 0x1p24f;
+                row_raise[i] = 0.f;
+                if constexpr (RAISED) {
+                    sum += __shfl_xor(sum, 16);
+                    sum += __shfl_xor(sum, 32);
+                    row_raise[i] = -128.f * sum * row_scale[i];
+                    row_scale[i] *= 0x1p24f;
+                }
             }
+        }
+    }
+
+    // The weights w (fp32 rows: w + wl) of K tiles from t on from their scores, with l,
+    // and with M and acc where the reference has to move.  edge: some row does not
+    // attend all keys; keys from key_end on are not this part's.  sc: each tile's K
+    // scale, log2 and reciprocal of its V scale.
+    template <int K>
+    __device__ __forceinline__ void weigh(const AttnArgs &a, const RowTile &rt, int t, bool edge, int key_end,
+                                          const float (&sc)[K][3], const f4 (&s)[K][NT][2], h8 (&w)[K][NT],
+                                          h8 (&wl)[K][F32 ? NT : 1], int n, int g) {
+        float x[K][NT][8], mx = -INFINITY;
+        const auto score = [&]() {
+            mx = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    const float c = row_scale[j] * sc[k][0];
+                    const float b = fmaf(row_raise[j], sc[k][0], sc[k][1] + (kHead - M[j]));
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[k][j][e] = fmaf(s[k][j][e >> 2][e & 3], c, b);
+                }
+            if (edge) {
+                asm volatile("");  // a branch: as selects the masks would be half of the loop's VALU work
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    const int row = rt.row0 + min(j * 16 + n, rt.rows - 1);
+                    const int pos = rt.kv_len - rt.new_len + row / a.group;
+                    const int lo = key_lo(a, pos), hi = min(key_hi(a, pos, rt.kv_len), key_end);
+#pragma unroll
+                    for (int k = 0; k < K; k++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const int key = (t + k) * 32 + g * 8 + e;
+                            x[k][j][e] = key >= lo && key < hi ? x[k][j][e] : -INFINITY;
+                        }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) mx = fmaxf(mx, x[k][j][e]);
+        };
+        score();
+        if (__any(mx > kLazy + kHead)) {
+            // a larger reference: from the scores again, as x may hold them against none
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                float m = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    const float c = row_scale[j] * sc[k][0], b = fmaf(row_raise[j], sc[k][0], sc[k][1]);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        m = fmaxf(m, x[k][j][e] == -INFINITY ? x[k][j][e] : fmaf(s[k][j][e >> 2][e & 3], c, b));
+                }
+                const float m1 = fmaxf(M[j], fmax16(m)), f = __builtin_amdgcn_exp2f(M[j] - m1);
+                M[j] = m1;
+                l[j] *= f;
+#pragma unroll
+                for (int d = 0; d < ND; d++) acc[j][d] *= f;
+            }
+            score();
+        }
+#pragma unroll
+        for (int k = 0; k < K; k++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float p = __builtin_amdgcn_exp2f(x[k][j][e]);
+                    sum += p;  // not the f16 weight: over a block of small V scale that may be 0
+                    w[k][j][e] = (_Float16)p;
+                    if constexpr (F32) wl[k][j][e] = (_Float16)(p - (float)w[k][j][e]);
+                }
+                l[j] = fmaf(sum, sc[k][2], l[j]);
+            }
+    }
+
+    // The four lanes of a row have the same M; its l is their sum.
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            l[j] += __shfl_xor(l[j], 16);
+            l[j] += __shfl_xor(l[j], 32);
         }
     }
 
@@ -247,32 +370,15 @@ struct Wave {
     __device__ __forceinline__ void attend(const AttnArgs &a, const RowTile &rt, int head, int t0, int t1,
                                            int step, int lane) {
         const int n = lane & 15, g = lane >> 4;
-        const int base_pos = rt.kv_len - rt.new_len;
-        const int last_row = rt.row0 + rt.rows - 1;
         // tiles inside [all_lo, all_hi] need no mask
-        const int all_lo = key_lo(a, base_pos + last_row / a.group);
-        const int all_hi = key_hi(a, base_pos + rt.row0 / a.group, rt.kv_len);
+        const int all_lo = key_lo(a, last_pos(a, rt)), all_hi = key_hi(a, first_pos(a, rt), rt.kv_len);
         const int32_t *table = a.tables + (size_t)rt.seq * a.max_pages;
         const int lg = a.pg.page_log2;
-        // the page, and its scales, of this wave's next 64 tiles: one a lane
-        int my_page = 0;
-        float my_ks = 0.f, my_lv = 0.f, my_rv = 0.f;
-        const auto load_pages = [&](int t) {
-            const int mine = t + lane * step;
-            const int p = mine < t1 ? table[mine >> (lg - 5)] : -1;
-            const bool ok = (unsigned)p < (unsigned)a.pg.n_pages;
-            my_page = ok ? p : 0;
-            const size_t b = (size_t)my_page * a.pg.n_kv + head;
-            const float raw = a.pg.vs[b];
-            const float vs = fmaxf(raw, kMinScale) + (raw - raw);  // NaN stays
-            my_ks = ok ? a.pg.ks[b] : 0.f;
-            my_lv = ok ? __builtin_amdgcn_logf(vs) : -INFINITY;  // no page: no weight
-            my_rv = ok && vs == vs ? 1.f / vs : 1.f;             // finite: a masked key's 0·rv stays 0
-        };
+        TilePages pages;
         const size_t lane_k = (size_t)((n >> 2) * 8 + (n & 3)) * HD + g * 16;
         const size_t lane_v = n * 32 + g * 8;
         const auto block = [&](int t, int i) {  // the quants of tile t, the wave's i-th
-            const int page = __builtin_amdgcn_readlane(my_page, i % 64);
+            const int page = __builtin_amdgcn_readlane(pages.page, i % 64);
             return ((((size_t)page * a.pg.n_kv + head) << (lg - 5)) + (t & ((1 << (lg - 5)) - 1))) * (32 * HD);
         };
         u4 kr[NC][2];
@@ -285,18 +391,19 @@ struct Wave {
                 for (int h = 0; h < 2; h++) kr[c][h] = load<STREAM, u4>(p + c * 64 + h * 4 * HD);
         };
         if (t0 >= t1) return;
-        load_pages(t0);
+        pages.load(a, table, head, t0, step, t1);
         size_t blk = block(t0, 0);
         load_k(blk);
         // One tile.  Its V and then the next tile's K are on their way while it is
         // worked on; the last tile has a copy of this code without that K, as a
         // load under a condition would be waited for at once.
         const auto tile = [&](int i, int t, auto more) {
-            const float tks = lane_f(my_ks, i % 64), lv = lane_f(my_lv, i % 64), rv = lane_f(my_rv, i % 64);
+            float sc[1][3];
+            pages.scales(i % 64, sc[0]);
             const int8_t *vp = a.pg.vq + blk + lane_v;
 #pragma unroll
             for (int d = 0; d < ND; d++) vr[d] = load<STREAM, u2>(vp + d * 16 * 32);
-            f4 s[NT][2];
+            f4 sk[1][NT][2], (&s)[NT][2] = sk[0];
 #pragma unroll
             for (int j = 0; j < NT; j++) s[j][0] = s[j][1] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -319,61 +426,12 @@ struct Wave {
                     }
                 }
             if constexpr (decltype(more)::value) {
-                if (i % 64 == 63) load_pages(t + step);
+                if (i % 64 == 63) pages.load(a, table, head, t + step, step, t1);
                 blk = block(t + step, i + 1);
                 load_k(blk);
             }
-            float x[NT][8], mx = -INFINITY;
-            const bool edge = t * 32 < all_lo || t * 32 + 32 > all_hi;
-            const auto weights = [&]() {
-                mx = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    const float c = row_scale[j] * tks, b = fmaf(row_raise[j], tks, lv + (kHead - M[j]));
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[j][e] = fmaf(s[j][e >> 2][e & 3], c, b);
-                    if (edge) {
-                        const int row = rt.row0 + min(j * 16 + n, rt.rows - 1);
-                        const int pos = base_pos + row / a.group;
-                        const int lo = key_lo(a, pos), hi = key_hi(a, pos, rt.kv_len), key = t * 32 + g * 8;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) x[j][e] = key + e >= lo && key + e < hi ? x[j][e] : -INFINITY;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; e++) mx = fmaxf(mx, x[j][e]);
-                }
-            };
-            weights();
-            if (__any(mx > kLazy + kHead)) {
-                // a larger reference: from the scores again, as x may hold them against none
-#pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    const float c = row_scale[j] * tks, b = fmaf(row_raise[j], tks, lv);
-                    float m = -INFINITY;
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        m = fmaxf(m, x[j][e] == -INFINITY ? x[j][e] : fmaf(s[j][e >> 2][e & 3], c, b));
-                    const float m1 = fmaxf(M[j], fmax16(m)), f = __builtin_amdgcn_exp2f(M[j] - m1);
-                    M[j] = m1;
-                    l[j] *= f;
-#pragma unroll
-                    for (int d = 0; d < ND; d++) acc[j][d] *= f;
-                }
-                weights();
-            }
-            h8 w[NT], wl[F32 ? NT : 1];
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-                float sum = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float p = __builtin_amdgcn_exp2f(x[j][e]);
-                    sum += p;  // not the f16 weight: over a block of small V scale that may be 0
-                    w[j][e] = (_Float16)p;
-                    if constexpr (F32) wl[j][e] = (_Float16)(p - (float)w[j][e]);
-                }
-                l[j] = fmaf(sum, rv, l[j]);
-            }
+            h8 wk[1][NT], wlk[1][F32 ? NT : 1], (&w)[NT] = wk[0], (&wl)[F32 ? NT : 1] = wlk[0];
+            weigh<1>(a, rt, t, t * 32 < all_lo || t * 32 + 32 > all_hi, INT32_MAX, sc, sk, wk, wlk, n, g);
 #pragma unroll
             for (int d = 0; d < ND; d++) {
                 const h8 v = quants_f16(vr[d].x, vr[d].y);
@@ -387,11 +445,7 @@ struct Wave {
         int i = 0, t = t0;
         for (; t + step < t1; i++, t += step) tile(i, t, std::true_type{});
         tile(i, t, std::false_type{});
-#pragma unroll
-        for (int j = 0; j < NT; j++) {  // the lanes of a row have the same M
-            l[j] += __shfl_xor(l[j], 16);
-            l[j] += __shfl_xor(l[j], 32);
-        }
+        finish();
     }
 };
 
@@ -423,7 +477,7 @@ __global__ __launch_bounds__(kFewWaves * 64, HD == 128 ? 3 : HD == 256 ? 2 : 1) 
     if (split >= ks.parts) return;
     const int t0 = ks.t0 + split * ks.per, t1 = min(t0 + ks.per, ks.t1);
     Wave<T, HD, 1> w;
-    w.load_q(a, rt, head, n, g);
+    w.template load_q<true>(a, rt, head, n, g);
     w.template attend<true>(a, rt, head, t0 + wave, t1, kFewWaves, lane);
     if (g == 0) {
         ml_s[wave][0][n] = w.M[0];
@@ -465,33 +519,236 @@ __global__ __launch_bounds__(kFewWaves * 64, HD == 128 ? 3 : HD == 256 ? 2 : 1) 
     }
 }
 
-// Many rows: each wave has 16·NT rows of its own and walks all keys of its part.
-constexpr int kManyWaves = 4;
+// Many rows: a workgroup's waves have 16·NT rows each and share the keys.  A step
+// of kStep 32-key tiles is turned into f16 once, by all waves, into LDS.
+// The two waves of a SIMD take turns: while one multiplies (the last step's P·V,
+// then this step's Q·K, with the conversion of its share of the next quants in
+// the products' shadow) the other weighs its scores, with a barrier at each
+// change, so that the matrix cores and the vector units both have work all the
+// time.  Phase 2t+w is the multiplication of step t for waves of group w = 0, 1,
+// phase 2t+1+w their weighing.  K(t+1) and V(t) are stored in the phases 2t and
+// 2t+1: complete before phase 2t+2, which reads them first, and over K(t-1) and
+// V(t-2), which phase 2t-1 read last, so two buffers of each do.
+//   K [key][HD]: the 16-byte units of a row are stored at unit ^ swizzle(key), so
+//                that the 16 keys of a fragment read fall on different banks
+//   V [tile][dim][32 keys]: a fragment is one kilobyte, its four units of a dim
+//                likewise exchanged
 template <typename T, int HD>
-constexpr int many_tiles() {  // column tiles that the registers hold
-    return HD == 128 ? 2 : HD == 256 ? (sizeof(T) == 2 ? 2 : 1) : 1;
-}
+struct Many {
+    static constexpr bool F32 = sizeof(T) == 4;
+    // the accumulator (64·NT·HD/128 registers) and q bound the rows of a wave
+    static constexpr int NT = HD == 128 && !F32 ? 2 : 1;
+    static constexpr int kWaves = HD == 512 ? 4 : 8;  // 512 dims take the registers of two
+    static constexpr int kRows = kWaves * NT * 16;
+    static constexpr int kStep = HD == 128 || (HD == 256 && F32) ? 2 : 1;
+    static constexpr int kThreads = kWaves * 64;
+    static constexpr int kGroups = kWaves / 4;
+    static constexpr int kLoads = kStep * 2 * HD / kThreads;  // 16-byte loads a thread, for K and for V
+    static_assert(kLoads * kThreads == kStep * 2 * HD && 2 * HD % 64 == 0, "whole waves load a tile");
+    static constexpr int kFrags = kStep * HD / 16;  // fragments of a step's K, and of its V
+    static constexpr int kAhead = 4;                // fragment reads under way
+    struct Lds {
+        h8 k[2][kStep][32][HD / 8];
+        h8 v[2][kStep][HD][4];
+    };
+    static __device__ __forceinline__ int swizzle_v(int dim) { return (dim >> 2 & 3) ^ (dim & 2); }
+    static __device__ __forceinline__ int swizzle(int key) { return (key & 3) | (key >> 3 & 3) << 2; }
+};
 
 template <typename T, int HD>
-__global__ __launch_bounds__(kManyWaves * 64, HD < 512 ? 2 : 1) void paged_attn_many_kernel(AttnArgs a, int n_wgs) {
-    constexpr int NT = many_tiles<T, HD>();
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+__global__ __launch_bounds__((Many<T, HD>::kThreads), (Many<T, HD>::kWaves / 4)) void paged_attn_many_kernel(AttnArgs a, int n_tiles) {
+    using C = Many<T, HD>;
+    constexpr int NT = C::NT, KT = C::kStep;
+    __shared__ __align__(16) typename C::Lds lds;
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+    // in a scalar register: what follows from it, barriers among it, branches for the
+    // whole wave
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // XCD = id % 8 takes heads congruent to it, so its L2 holds their pages; the
     // last tiles, which attend most keys, go first
-    const int split = blockIdx.y % a.many_splits;
-    const int head = blockIdx.x % a.pg.n_kv, wg = n_wgs - 1 - blockIdx.x / a.pg.n_kv;
+    const int split = blockIdx.y;
+    const int head = blockIdx.x % a.pg.n_kv, id = n_tiles - 1 - blockIdx.x / a.pg.n_kv;
     RowTile rt;
-    if (!many_rows<NT * 16>(a, wg * kManyWaves + wave, &rt)) return;
+    if (!many_rows<C::kRows>(a, id, &rt)) return;
     const KeySpan ks = key_span(a, rt, a.many_splits, a.many_per);
     if (split >= ks.parts) return;
     const int t0 = ks.t0 + split * ks.per, t1 = min(t0 + ks.per, ks.t1);
+
+    // this wave's rows
+    RowTile wt = rt;
+    const bool idle = wave * NT * 16 >= rt.rows;
+    wt.row0 = rt.row0 + (idle ? 0 : wave * NT * 16);
+    wt.rows = idle ? 1 : min(rt.rows - wave * NT * 16, NT * 16);
+    const int all_lo = key_lo(a, last_pos(a, wt)), all_hi = min(key_hi(a, first_pos(a, wt), rt.kv_len), t1 * 32);
     Wave<T, HD, NT> w;
-    w.load_q(a, rt, head, n, g);
-    w.template attend<false>(a, rt, head, t0, t1, 1, lane);
+    w.template load_q<false>(a, wt, head, n, g);
+
+    const int32_t *table = a.tables + (size_t)rt.seq * a.max_pages;
+    const int lg = a.pg.page_log2 - 5;  // tiles of a page, log2
+    // What this wave loads of a step: kLoads pieces of K and V, each of one tile.
+    u4 kr[C::kLoads], vr[C::kLoads];
+    int page_k[C::kLoads], page_v[C::kLoads];
+    const auto tile_of = [&](int step, int p) {  // past the end: the last one again, unused
+        return min(t0 + step * KT + (p * C::kThreads + wave * 64) / (2 * HD), t1 - 1);
+    };
+    int pages[C::kLoads];  // of 64 steps: one a lane
+    // Steps are looked up one after another.
+    const auto look_up = [&](int step, int (&page)[C::kLoads]) {
+        if ((step & 63) == 0) {
+#pragma unroll
+            for (int p = 0; p < C::kLoads; p++) {
+                const int v = table[tile_of(step + lane, p) >> lg];
+                pages[p] = (unsigned)v < (unsigned)a.pg.n_pages ? v : 0;  // none: any, as it weighs nothing
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < C::kLoads; p++) page[p] = __builtin_amdgcn_readlane(pages[p], step & 63);
+    };
+    const auto quants_at = [&](int step, int p, int page) {
+        return ((((size_t)page * a.pg.n_kv + head) << lg) + (tile_of(step, p) & ((1 << lg) - 1))) * (32 * HD) +
+               (size_t)((p * C::kThreads + tid) % (2 * HD)) * 16;
+    };
+    const auto load_k = [&](int step) {
+#pragma unroll
+        for (int p = 0; p < C::kLoads; p++)
+            kr[p] = *reinterpret_cast<const u4 *>(a.pg.kq + quants_at(step, p, page_k[p]));
+    };
+    const auto load_v = [&](int step) {
+#pragma unroll
+        for (int p = 0; p < C::kLoads; p++)
+            vr[p] = *reinterpret_cast<const u4 *>(a.pg.vq + quants_at(step, p, page_v[p]));
+    };
+    // Piece i of the conversion: 8 quants of K(step + 1) or V(step) into LDS.
+    const auto convert = [&](int step, int i) {
+        const int p = i / 4, half = i & 1;
+        const int at = p * C::kThreads + tid, tile = at / (2 * HD), u = at % (2 * HD);
+        if ((i & 2) == 0) {
+            const int key = u / (HD / 16), c = u % (HD / 16) * 2 + half;  // 16 dims of a key
+            lds.k[(step + 1) & 1][tile][key][c ^ C::swizzle(key)] =
+                half ? quants_f16(kr[p].z, kr[p].w) : quants_f16(kr[p].x, kr[p].y);
+        } else {
+            const int dim = u / 2, c = u % 2 * 2 + half;  // 16 keys of a dim
+            lds.v[step & 1][tile][dim][c ^ C::swizzle_v(dim)] =
+                half ? quants_f16(vr[p].z, vr[p].w) : quants_f16(vr[p].x, vr[p].y);
+        }
+    };
+    h8 hi[KT][NT], lo[KT][C::F32 ? NT : 1];  // the last weighed step's weights
+    f4 s[KT][NT][2];                         // the last multiplied step's scores
+    // Fragment i of V(step): tile i / (HD/16), dims i % (HD/16).
+    const auto read_v = [&](int step, int i) {
+        return lds.v[step & 1][i / (HD / 16)][i % (HD / 16) * 16 + n][g ^ C::swizzle_v(n)];
+    };
+    const auto multiply_v = [&](int i, h8 f) {
+        const int k = i / (HD / 16), d = i % (HD / 16);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            w.acc[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, hi[k][j], w.acc[j][d], 0, 0, 0);
+            if constexpr (C::F32)
+                w.acc[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, lo[k][j], w.acc[j][d], 0, 0, 0);
+        }
+    };
+    // Fragment i of K(step): half h of tile k against 32 dims, the dims outermost so that
+    // products of one sum lie apart.
+    const auto read_k = [&](int step, int i) {
+        const int h = i % 2, k = i / 2 % KT, ce = i / 2 / KT;
+        // swizzle(key) is n; the units it exchanges lie within 16
+        const int key = (n >> 2) * 8 + h * 4 + (n & 3), in16 = ce / 2 % 2 * 8 + g * 2 + ce % 2;
+        return lds.k[step & 1][k][key][ce / 4 * 16 + (in16 ^ n)];
+    };
+    const auto multiply_k = [&](int i, h8 f) {
+        const int h = i % 2, k = i / 2 % KT, ce = i / 2 / KT;
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const f4 sum = ce == 0 ? f4{0.f, 0.f, 0.f, 0.f} : s[k][j][h];
+            s[k][j][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, w.qa[j][ce / 2][ce % 2], sum, 0, 0, 0);
+            if constexpr (C::F32)
+                s[k][j][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, w.ql[j][ce / 2][ce % 2], s[k][j][h], 0, 0, 0);
+        }
+    };
+    const auto load_next = [&](int t) {
+        load_k(t + 3);
+        load_v(t + 2);
+#pragma unroll
+        for (int p = 0; p < C::kLoads; p++) page_v[p] = page_k[p];
+        look_up(t + 4, page_k);
+    };
+    // A phase of products: P(t)·V(t) when there is one, Q·K(t+1), with the pieces of the
+    // conversion after it spread among them.  The order is as written (the
+    // sched_barriers): left alone the compiler waits for each fragment at once, for
+    // longer than its products take.
+    const auto multiply = [&](int t, auto with_v) {
+        constexpr int NV = decltype(with_v)::value ? C::kFrags : 0, N = NV + C::kFrags, A = C::kAhead;
+        constexpr int kPieces = C::kLoads * 4, kEvery = C::kFrags / kPieces;
+        const auto read = [&](int i) { return i < NV ? read_v(t, i) : read_k(t + 1, i - NV); };
+        h8 f[A];
+#pragma unroll
+        for (int i = 0; i < A; i++) f[i] = read(i);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (i < NV) multiply_v(i, f[i % A]);
+            else multiply_k(i - NV, f[i % A]);
+            if (i + A < N) f[i % A] = read(i + A);
+            // in the last products' shadow: the quants have had the longest time to come
+            if (i >= N - C::kFrags && (i - (N - C::kFrags)) % kEvery == kEvery - 1)
+                convert(t + 1, (i - (N - C::kFrags)) / kEvery);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load_next(t);
+    };
+    const int steps = (t1 - t0 + KT - 1) / KT, group = wave / 4;
+    if (steps > 0) {
+        look_up(0, page_k);
+        load_k(0);
+#pragma unroll
+        for (int p = 0; p < C::kLoads; p++) {
+            convert(-1, p * 4);
+            convert(-1, p * 4 + 1);
+        }
+#pragma unroll
+        for (int p = 0; p < C::kLoads; p++) page_v[p] = page_k[p];
+        look_up(1, page_k);
+        load_k(1);
+        load_v(0);
+        // registers: K(1), V(0)
+#pragma unroll
+        for (int p = 0; p < C::kLoads; p++) page_v[p] = page_k[p];
+        look_up(2, page_k);
+        __syncthreads();
+        if (group == 1) __syncthreads();
+        multiply(-1, std::false_type{});
+        __syncthreads();
+    }
+    if (idle) {  // no rows: only its share of the conversion, at the same barriers
+        for (int t = 0; t < steps; t++) {
+            const bool more = t + 1 < steps;
+            if (group == 0 || more) __syncthreads();
+#pragma unroll
+            for (int i = 0; i < C::kLoads * 4; i++) convert(t + 1, i);
+            load_next(t);
+            if (more) __syncthreads();
+        }
+        return;
+    }
+    TilePages tiles;
+    // Steps that a wave's rows do not reach weigh nothing, like the copies past the end.
+    for (int t = 0; t < steps; t++) {
+        const int at = t0 + t * KT, turn = t * KT % 64;
+        if (turn == 0) tiles.load(a, table, head, at, 1, t1);
+        float sc[KT][3];
+#pragma unroll
+        for (int k = 0; k < KT; k++) tiles.scales(turn + k, sc[k]);
+        w.template weigh<KT>(a, wt, at, at * 32 < all_lo || (at + KT) * 32 > all_hi, t1 * 32, sc, s, hi, lo, n, g);
+        const bool more = t + 1 < steps;
+        if (group == 0 || more) __syncthreads();
+        multiply(t, std::true_type{});
+        if (more) __syncthreads();
+    }
+    w.finish();
 #pragma unroll
     for (int j = 0; j < NT; j++) {
-        const int row = rt.row0 + j * 16 + n;
-        if (j * 16 + n >= rt.rows) continue;
+        const int row = wt.row0 + j * 16 + n;
+        if (j * 16 + n >= wt.rows) continue;
         const int tok = rt.tok0 + row / a.group, qh = head * a.group + row % a.group;
         if (ks.parts == 1) {
             const float inv = inverse(w.l[j]);
@@ -507,38 +764,44 @@ __global__ __launch_bounds__(kManyWaves * 64, HD < 512 ? 2 : 1) void paged_attn_
     }
 }
 
-// Joins the parts of a row tile's rows, in their order: a wave a row, its lanes
-// first share out the parts' references and sums, then the dims.
+// Joins the parts of a row, in their order: a wave a row.  Its lanes share out the
+// parts' references and sums, then the dims, four parts' loads in flight.
 template <typename T, int HD>
-__device__ __forceinline__ void join_rows(const AttnArgs &a, const RowTile &rt, int head, int parts) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int i = wave; i < rt.rows; i += 4) {
-        const int r = rt.row0 + i;
-        const int tok = rt.tok0 + r / a.group, qh = head * a.group + r % a.group;
-        const size_t prow = ((size_t)tok * a.n_q + qh) * a.part_slots;
-        float m = kNoMax, l = 0.f, o[HD / 64];
-        for (int s = lane; s < parts; s += 64) m = fmaxf(m, a.part_ml[prow + s].x);
+__device__ __forceinline__ void join_row(const AttnArgs &a, const RowTile &rt, int head, int i, int parts) {
+    const int lane = threadIdx.x & 63, r = rt.row0 + i;
+    const int tok = rt.tok0 + r / a.group, qh = head * a.group + r % a.group;
+    const size_t prow = ((size_t)tok * a.n_q + qh) * a.part_slots;
+    float m = kNoMax, l = 0.f, o[HD / 64];
+    for (int s = lane; s < parts; s += 64) m = fmaxf(m, a.part_ml[prow + s].x);
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
 #pragma unroll
-        for (int d = 0; d < HD / 64; d++) o[d] = 0.f;
-        for (int b = 0; b < parts; b += 64) {
-            const float2 ml = b + lane < parts ? a.part_ml[prow + b + lane] : make_float2(kNoMax, 0.f);
-            const float mine = __builtin_amdgcn_exp2f(ml.x - m), ls = ml.y * mine;
-            const int e = min(parts - b, 64);
-            for (int s = 0; s < e; s++) {
-                const float f = lane_f(mine, s);
-                l += lane_f(ls, s);
+    for (int d = 0; d < HD / 64; d++) o[d] = 0.f;
+    for (int b = 0; b < parts; b += 64) {
+        const float2 ml = b + lane < parts ? a.part_ml[prow + b + lane] : make_float2(kNoMax, 0.f);
+        const float mine = b + lane < parts ? __builtin_amdgcn_exp2f(ml.x - m) : 0.f, ls = ml.y * mine;
+        const int e = min(parts - b, 64);
+        for (int s = 0; s < e; s += 4) {
+            float v[4][HD / 64];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
 #pragma unroll
                 for (int d = 0; d < HD / 64; d++)
-                    o[d] = fmaf(a.part[(prow + b + s) * HD + d * 64 + lane], f, o[d]);
+                    v[k][d] = a.part[(prow + b + min(s + k, e - 1)) * HD + d * 64 + lane];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (s + k >= e) break;
+                const float f = lane_f(mine, s + k);
+                l += lane_f(ls, s + k);
+#pragma unroll
+                for (int d = 0; d < HD / 64; d++) o[d] = fmaf(v[k][d], f, o[d]);
             }
         }
-        const float inv = inverse(l);
-        T *dst = static_cast<T *>(a.out) + (size_t)tok * a.out_stride + (size_t)qh * HD;
-#pragma unroll
-        for (int d = 0; d < HD / 64; d++) dst[d * 64 + lane] = (T)(o[d] * inv);
     }
+    const float inv = inverse(l);
+    T *dst = static_cast<T *>(a.out) + (size_t)tok * a.out_stride + (size_t)qh * HD;
+#pragma unroll
+    for (int d = 0; d < HD / 64; d++) dst[d * 64 + lane] = (T)(o[d] * inv);
 }
 
 template <typename T, int HD>
@@ -546,23 +809,25 @@ __global__ __launch_bounds__(256) void paged_attn_join_few_kernel(AttnArgs a) {
     RowTile rt;
     if (!few_rows(a, blockIdx.x, &rt)) return;
     const KeySpan ks = key_span(a, rt, a.few_splits, a.few_per);
-    if (ks.parts > 1) join_rows<T, HD>(a, rt, blockIdx.y, ks.parts);
+    const int i = blockIdx.z * 4 + (threadIdx.x >> 6);
+    if (ks.parts > 1 && i < rt.rows) join_row<T, HD>(a, rt, blockIdx.y, i, ks.parts);
 }
 
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void paged_attn_join_many_kernel(AttnArgs a) {
     RowTile rt;
-    if (!many_rows<many_tiles<T, HD>() * 16>(a, blockIdx.x, &rt)) return;
+    if (!many_rows<Many<T, HD>::kRows>(a, blockIdx.x, &rt)) return;
     const KeySpan ks = key_span(a, rt, a.many_splits, a.many_per);
-    if (ks.parts > 1) join_rows<T, HD>(a, rt, blockIdx.y, ks.parts);
+    const int i = blockIdx.z * 4 + (threadIdx.x >> 6);
+    if (ks.parts > 1 && i < rt.rows) join_row<T, HD>(a, rt, blockIdx.y, i, ks.parts);
 }
 
 // How a call is laid out: which kernels run, and into how many parts at most
 // they cut the keys of a row.
-constexpr int kFewWgs = 1024;
+constexpr int kFewWgs = 1024, kManyWgs = 256;
 struct Layout {
     bool few, many;
-    int few_splits, many_splits, many_wgs;
+    int few_splits, many_splits, many_tiles;
 };
 
 // Parts of 256 keys or more, so many that `units` workgroups of one part each
@@ -583,10 +848,12 @@ Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f1
     y.few_splits = y.many_splits = 1;
     if (y.few) y.few_splits = splits_for((long long)n_seqs * n_kv, kFewWgs, max_kv);
     if (y.many) {
-        const int bm = 16 * (head_dim == 128 ? 2 : head_dim == 256 ? (f16 ? 2 : 1) : 1);
-        const long long tiles = (long long)n_tokens * group / bm + n_seqs;
-        y.many_wgs = (int)((tiles + kManyWaves - 1) / kManyWaves);
-        y.many_splits = splits_for((long long)y.many_wgs * n_kv, 512, max_kv);
+        const int bm = head_dim == 128 ? (f16 ? Many<_Float16, 128>::kRows : Many<float, 128>::kRows)
+                       : head_dim == 256 ? (f16 ? Many<_Float16, 256>::kRows : Many<float, 256>::kRows)
+                                         : (f16 ? Many<_Float16, 512>::kRows : Many<float, 512>::kRows);
+        y.many_tiles = (int)((long long)n_tokens * group / bm) + n_seqs;
+        // about as many tiles as one request with all rows has: the room for more is mostly empty
+        y.many_splits = splits_for(((long long)n_tokens * group / bm + 1) * n_kv, kManyWgs, max_kv);
     }
     return y;
 }
@@ -594,8 +861,8 @@ Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f1
 template <typename T, int HD>
 int launch(hipStream_t st, const AttnArgs &a, const Layout &y) {
     if (y.many) {
-        hipLaunchKernelGGL((paged_attn_many_kernel<T, HD>), dim3(y.many_wgs * a.pg.n_kv, a.many_splits),
-                           dim3(kManyWaves * 64), 0, st, a, y.many_wgs);
+        hipLaunchKernelGGL((paged_attn_many_kernel<T, HD>), dim3(y.many_tiles * a.pg.n_kv, a.many_splits),
+                           dim3(Many<T, HD>::kThreads), 0, st, a, y.many_tiles);
         SGQ_HIP(hipGetLastError());
     }
     if (y.few) {
@@ -605,11 +872,13 @@ int launch(hipStream_t st, const AttnArgs &a, const Layout &y) {
     }
     if (y.many && a.many_splits > 1) {
         hipLaunchKernelGGL((paged_attn_join_many_kernel<T, HD>),
-                           dim3(y.many_wgs * kManyWaves, a.pg.n_kv), dim3(256), 0, st, a);
+                           dim3(y.many_tiles, a.pg.n_kv, Many<T, HD>::kRows / 4), dim3(256), 0, st, a);
         SGQ_HIP(hipGetLastError());
     }
     if (y.few && a.few_splits > 1) {
-        hipLaunchKernelGGL((paged_attn_join_few_kernel<T, HD>), dim3(a.n_seqs, a.pg.n_kv), dim3(256), 0, st, a);
+        const int rows = std::min(a.max_new * a.group, kFewRows);
+        hipLaunchKernelGGL((paged_attn_join_few_kernel<T, HD>), dim3(a.n_seqs, a.pg.n_kv, (rows + 3) / 4),
+                           dim3(256), 0, st, a);
         SGQ_HIP(hipGetLastError());
     }
     return SGQ_OK;
