@@ -37,12 +37,16 @@ struct AttnArgs {
     void *out;
     uint64_t q_stride, out_stride;
     const int32_t *tables, *kv_lens, *cu;
-    float *part;      // [row][split][hd]
-    float2 *part_ml;  // [row][split] (M, l)
+    // the parts' sums [row][part][hd] and (M, l) [row][part]: rows (request, kv head, row)
+    // of few rows, (cut tile, kv head, row of the tile) or (token, head) of many
+    float *few_part, *many_part;
+    float2 *few_ml, *many_ml;
     int max_pages, n_seqs, n_tokens, n_q, group, max_new, window;
     int few_splits, many_splits;  // parts at most, of requests with few and with many rows
     int few_per, many_per;        // their length in 32-key tiles, if that makes no more of them
-    int part_slots;               // parts that the workspace holds for a row
+    int many_tiles, many_whole;   // row tiles, and how many of the first (in launch order) stay whole
+    int few_cap;                  // rows a request of few has at most
+    bool many_by_token;           // whichever is fewer rows
     bool few;                     // requests with few rows go to their own kernel
     float scale_log2;
 };
@@ -458,6 +462,19 @@ __device__ __forceinline__ void store4(_Float16 *p, float4 v) {
 // a row that attends nothing is zero
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
+// A row's place in the workspace.
+__device__ __forceinline__ size_t few_row(const AttnArgs &a, const RowTile &rt, int head, int i) {
+    return ((size_t)rt.seq * a.pg.n_kv + head) * a.few_cap + i;
+}
+template <int BM>
+__device__ __forceinline__ size_t many_row(const AttnArgs &a, const RowTile &rt, int cut_tile, int head, int i) {
+    if (a.many_by_token) {
+        const int r = rt.row0 + i;
+        return (size_t)(rt.tok0 + r / a.group) * a.n_q + head * a.group + r % a.group;
+    }
+    return ((size_t)cut_tile * a.pg.n_kv + head) * BM + i;
+}
+
 // Few rows: one request and kv head against one part of the keys, the tiles dealt
 // to 4 waves in turn and their sums joined in LDS in wave order.
 constexpr int kFewWaves = 4;
@@ -496,7 +513,7 @@ __global__ __launch_bounds__(kFewWaves * 64, HD == 128 ? 3 : HD == 256 ? 2 : 1) 
     for (int i = 0; i < kFewWaves; i++)
         ol += ml_s[i][1][orow] * __builtin_amdgcn_exp2f(ml_s[i][0][orow] - om);
     const int otok = rt.tok0 + orow / a.group, oh = head * a.group + orow % a.group;
-    const size_t prow = ((size_t)otok * a.n_q + oh) * a.part_slots + split;
+    const size_t prow = few_row(a, rt, head, orow) * a.few_splits + split;
     const float inv = inverse(ol);
 #pragma unroll
     for (int c = 0; c < NC; c++) {
@@ -512,8 +529,8 @@ __global__ __launch_bounds__(kFewWaves * 64, HD == 128 ? 3 : HD == 256 ? 2 : 1) 
                 store4(static_cast<T *>(a.out) + (size_t)otok * a.out_stride + (size_t)oh * HD + c * 64 + od,
                        scaled(o, inv));
             } else {
-                store4(a.part + prow * HD + c * 64 + od, scaled(o, 1.f));
-                if (c == 0 && od == 0) a.part_ml[prow] = make_float2(om, ol);
+                store4(a.few_part + prow * HD + c * 64 + od, scaled(o, 1.f));
+                if (c == 0 && od == 0) a.few_ml[prow] = make_float2(om, ol);
             }
         }
     }
@@ -540,7 +557,7 @@ struct Many {
     static constexpr int NT = HD == 128 && !F32 ? 2 : 1;
     static constexpr int kWaves = HD == 512 ? 4 : 8;  // 512 dims take the registers of two
     static constexpr int kRows = kWaves * NT * 16;
-    static constexpr int kStep = HD == 128 || (HD == 256 && F32) ? 2 : 1;
+    static constexpr int kStep = HD == 128 ? 2 : 1;
     static constexpr int kThreads = kWaves * 64;
     static constexpr int kGroups = kWaves / 4;
     static constexpr int kLoads = kStep * 2 * HD / kThreads;  // 16-byte loads a thread, for K and for V
@@ -551,12 +568,12 @@ struct Many {
         h8 k[2][kStep][32][HD / 8];
         h8 v[2][kStep][HD][4];
     };
-    static __device__ __forceinline__ int swizzle_v(int dim) { return (dim >> 2 & 3) ^ (dim & 2); }
+    static __device__ __forceinline__ int swizzle_v(int dim) { return -(dim >> 2) & 3; }
     static __device__ __forceinline__ int swizzle(int key) { return (key & 3) | (key >> 3 & 3) << 2; }
 };
 
 template <typename T, int HD>
-__global__ __launch_bounds__((Many<T, HD>::kThreads), (Many<T, HD>::kWaves / 4)) void paged_attn_many_kernel(AttnArgs a, int n_tiles) {
+__global__ __launch_bounds__((Many<T, HD>::kThreads), (Many<T, HD>::kWaves / 4)) void paged_attn_many_kernel(AttnArgs a) {
     using C = Many<T, HD>;
     constexpr int NT = C::NT, KT = C::kStep;
     __shared__ __align__(16) typename C::Lds lds;
@@ -566,11 +583,14 @@ __global__ __launch_bounds__((Many<T, HD>::kThreads), (Many<T, HD>::kWaves / 4))
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // XCD = id % 8 takes heads congruent to it, so its L2 holds their pages; the
     // last tiles, which attend most keys, go first
-    const int split = blockIdx.y;
-    const int head = blockIdx.x % a.pg.n_kv, id = n_tiles - 1 - blockIdx.x / a.pg.n_kv;
+    const int n_whole = a.many_whole * a.pg.n_kv, n_cut = (a.many_tiles - a.many_whole) * a.pg.n_kv;
+    const bool whole = (int)blockIdx.x < n_whole;
+    const int y = whole ? blockIdx.x : (blockIdx.x - n_whole) % n_cut;
+    const int split = whole ? 0 : (blockIdx.x - n_whole) / n_cut;
+    const int head = y % a.pg.n_kv, rank = y / a.pg.n_kv + (whole ? 0 : a.many_whole);
     RowTile rt;
-    if (!many_rows<C::kRows>(a, id, &rt)) return;
-    const KeySpan ks = key_span(a, rt, a.many_splits, a.many_per);
+    if (!many_rows<C::kRows>(a, a.many_tiles - 1 - rank, &rt)) return;
+    const KeySpan ks = key_span(a, rt, whole ? 1 : a.many_splits, a.many_per);
     if (split >= ks.parts) return;
     const int t0 = ks.t0 + split * ks.per, t1 = min(t0 + ks.per, ks.t1);
 
@@ -756,10 +776,11 @@ __global__ __launch_bounds__((Many<T, HD>::kThreads), (Many<T, HD>::kWaves / 4))
 #pragma unroll
             for (int d = 0; d < HD / 16; d++) store4(dst + d * 16, scaled(w.acc[j][d], inv));
         } else {
-            const size_t prow = ((size_t)tok * a.n_q + qh) * a.part_slots + split;
+            const size_t prow =
+                many_row<C::kRows>(a, rt, rank - a.many_whole, head, row - rt.row0) * a.many_splits + split;
 #pragma unroll
-            for (int d = 0; d < HD / 16; d++) store4(a.part + prow * HD + d * 16 + g * 4, scaled(w.acc[j][d], 1.f));
-            if (g == 0) a.part_ml[prow] = make_float2(w.M[j], w.l[j]);
+            for (int d = 0; d < HD / 16; d++) store4(a.many_part + prow * HD + d * 16 + g * 4, scaled(w.acc[j][d], 1.f));
+            if (g == 0) a.many_ml[prow] = make_float2(w.M[j], w.l[j]);
         }
     }
 }
@@ -767,18 +788,18 @@ __global__ __launch_bounds__((Many<T, HD>::kThreads), (Many<T, HD>::kWaves / 4))
 // Joins the parts of a row, in their order: a wave a row.  Its lanes share out the
 // parts' references and sums, then the dims, four parts' loads in flight.
 template <typename T, int HD>
-__device__ __forceinline__ void join_row(const AttnArgs &a, const RowTile &rt, int head, int i, int parts) {
+__device__ __forceinline__ void join_row(const AttnArgs &a, const RowTile &rt, int head, int i, int parts,
+                                         const float *part, const float2 *part_ml, size_t prow) {
     const int lane = threadIdx.x & 63, r = rt.row0 + i;
     const int tok = rt.tok0 + r / a.group, qh = head * a.group + r % a.group;
-    const size_t prow = ((size_t)tok * a.n_q + qh) * a.part_slots;
     float m = kNoMax, l = 0.f, o[HD / 64];
-    for (int s = lane; s < parts; s += 64) m = fmaxf(m, a.part_ml[prow + s].x);
+    for (int s = lane; s < parts; s += 64) m = fmaxf(m, part_ml[prow + s].x);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
 #pragma unroll
     for (int d = 0; d < HD / 64; d++) o[d] = 0.f;
     for (int b = 0; b < parts; b += 64) {
-        const float2 ml = b + lane < parts ? a.part_ml[prow + b + lane] : make_float2(kNoMax, 0.f);
+        const float2 ml = b + lane < parts ? part_ml[prow + b + lane] : make_float2(kNoMax, 0.f);
         const float mine = b + lane < parts ? __builtin_amdgcn_exp2f(ml.x - m) : 0.f, ls = ml.y * mine;
         const int e = min(parts - b, 64);
         for (int s = 0; s < e; s += 4) {
@@ -787,7 +808,7 @@ __device__ __forceinline__ void join_row(const AttnArgs &a, const RowTile &rt, i
             for (int k = 0; k < 4; k++)
 #pragma unroll
                 for (int d = 0; d < HD / 64; d++)
-                    v[k][d] = a.part[(prow + b + min(s + k, e - 1)) * HD + d * 64 + lane];
+                    v[k][d] = part[(prow + b + min(s + k, e - 1)) * HD + d * 64 + lane];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 if (s + k >= e) break;
@@ -810,24 +831,31 @@ __global__ __launch_bounds__(256) void paged_attn_join_few_kernel(AttnArgs a) {
     if (!few_rows(a, blockIdx.x, &rt)) return;
     const KeySpan ks = key_span(a, rt, a.few_splits, a.few_per);
     const int i = blockIdx.z * 4 + (threadIdx.x >> 6);
-    if (ks.parts > 1 && i < rt.rows) join_row<T, HD>(a, rt, blockIdx.y, i, ks.parts);
+    if (ks.parts > 1 && i < rt.rows)
+        join_row<T, HD>(a, rt, blockIdx.y, i, ks.parts, a.few_part, a.few_ml,
+                        few_row(a, rt, blockIdx.y, i) * a.few_splits);
 }
 
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void paged_attn_join_many_kernel(AttnArgs a) {
     RowTile rt;
-    if (!many_rows<Many<T, HD>::kRows>(a, blockIdx.x, &rt)) return;
+    if (!many_rows<Many<T, HD>::kRows>(a, a.many_tiles - 1 - a.many_whole - (int)blockIdx.x, &rt)) return;
     const KeySpan ks = key_span(a, rt, a.many_splits, a.many_per);
     const int i = blockIdx.z * 4 + (threadIdx.x >> 6);
-    if (ks.parts > 1 && i < rt.rows) join_row<T, HD>(a, rt, blockIdx.y, i, ks.parts);
+    if (ks.parts > 1 && i < rt.rows)
+        join_row<T, HD>(a, rt, blockIdx.y, i, ks.parts, a.many_part, a.many_ml,
+                        many_row<Many<T, HD>::kRows>(a, rt, blockIdx.x, blockIdx.y, i) * a.many_splits);
 }
 
 // How a call is laid out: which kernels run, and into how many parts at most
 // they cut the keys of a row.
-constexpr int kFewWgs = 1024, kManyWgs = 256;
+constexpr int kFewWgs = 1024;
+constexpr int kCus = 256;
+int few_cap(int max_new, int group) { return (int)std::min<long long>((long long)max_new * group, kFewRows); }
 struct Layout {
-    bool few, many;
-    int few_splits, many_splits, many_tiles;
+    bool few, many, many_by_token;
+    int few_splits, many_splits, many_tiles, many_whole;
+    uint64_t few_rows, many_rows;  // that may be cut
 };
 
 // Parts of 256 keys or more, so many that `units` workgroups of one part each
@@ -838,6 +866,22 @@ int splits_for(long long units, long long wanted, int max_kv) {
     return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
 }
 
+// Parts for `units` workgroups (below a round of the GPU, one a CU, or what is left
+// after whole rounds) of row tiles with `area` rows x dims.  A round costs its
+// tiles of 32 keys, 1.3 us each (1.1 to 2.1 measured), and four for its start;
+// joining p parts moves them twice, at 4 TB/s.
+int cut_for(int units, int area, int max_kv) {
+    const int tiles = (int)(((long long)max_kv + 31) / 32);
+    int best = 1;
+    double least = 0;
+    for (int p = 1; p <= 64 && (p == 1 || tiles / p >= 4); p++) {
+        const double rounds = (units * p + kCus - 1) / kCus;
+        const double us = 1.3 * rounds * ((tiles + p - 1) / p + 4) + (p > 1 ? 5 + 2e-6 * area * units * p : 0);
+        if (p == 1 || us < least) best = p, least = us;
+    }
+    return best;
+}
+
 Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f16, int max_new, int max_kv) {
     const int group = n_q / n_kv;
     Layout y{};
@@ -846,14 +890,25 @@ Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f1
     y.many = (long long)max_new * group > kFewRows;
     y.few = !y.many || n_seqs > 1;
     y.few_splits = y.many_splits = 1;
-    if (y.few) y.few_splits = splits_for((long long)n_seqs * n_kv, kFewWgs, max_kv);
+    if (y.few) {
+        y.few_splits = splits_for((long long)n_seqs * n_kv, kFewWgs, max_kv);
+        y.few_rows = (uint64_t)n_seqs * n_kv * few_cap(max_new, group);
+    }
     if (y.many) {
         const int bm = head_dim == 128 ? (f16 ? Many<_Float16, 128>::kRows : Many<float, 128>::kRows)
                        : head_dim == 256 ? (f16 ? Many<_Float16, 256>::kRows : Many<float, 256>::kRows)
                                          : (f16 ? Many<_Float16, 512>::kRows : Many<float, 512>::kRows);
         y.many_tiles = (int)((long long)n_tokens * group / bm) + n_seqs;
-        // about as many tiles as one request with all rows has: the room for more is mostly empty
-        y.many_splits = splits_for(((long long)n_tokens * group / bm + 1) * n_kv, kManyWgs, max_kv);
+        // The room for more tiles than one request with all rows has is mostly empty.
+        const int full = (int)((long long)n_tokens * group / bm) + 1;
+        y.many_whole = full * n_kv / kCus * kCus / n_kv + (y.many_tiles - full);
+        if (full * n_kv < kCus) y.many_whole = 0;
+        y.many_splits = cut_for((full * n_kv) % kCus, bm * head_dim, max_kv);
+        if (y.many_splits == 1) y.many_whole = y.many_tiles;
+        // with many requests most tiles are empty: then by token
+        y.many_rows = (uint64_t)(y.many_tiles - y.many_whole) * n_kv * bm;
+        y.many_by_token = y.many_rows > (uint64_t)n_tokens * n_q;
+        if (y.many_by_token) y.many_rows = (uint64_t)n_tokens * n_q;
     }
     return y;
 }
@@ -861,8 +916,8 @@ Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f1
 template <typename T, int HD>
 int launch(hipStream_t st, const AttnArgs &a, const Layout &y) {
     if (y.many) {
-        hipLaunchKernelGGL((paged_attn_many_kernel<T, HD>), dim3(y.many_tiles * a.pg.n_kv, a.many_splits),
-                           dim3(Many<T, HD>::kThreads), 0, st, a, y.many_tiles);
+        const int wgs = (a.many_whole + (a.many_tiles - a.many_whole) * a.many_splits) * a.pg.n_kv;
+        hipLaunchKernelGGL((paged_attn_many_kernel<T, HD>), dim3(wgs), dim3(Many<T, HD>::kThreads), 0, st, a);
         SGQ_HIP(hipGetLastError());
     }
     if (y.few) {
@@ -870,14 +925,13 @@ int launch(hipStream_t st, const AttnArgs &a, const Layout &y) {
                            dim3(kFewWaves * 64), 0, st, a);
         SGQ_HIP(hipGetLastError());
     }
-    if (y.many && a.many_splits > 1) {
+    if (y.many && a.many_splits > 1 && a.many_whole < a.many_tiles) {
         hipLaunchKernelGGL((paged_attn_join_many_kernel<T, HD>),
-                           dim3(y.many_tiles, a.pg.n_kv, Many<T, HD>::kRows / 4), dim3(256), 0, st, a);
+                           dim3(a.many_tiles - a.many_whole, a.pg.n_kv, Many<T, HD>::kRows / 4), dim3(256), 0, st, a);
         SGQ_HIP(hipGetLastError());
     }
     if (y.few && a.few_splits > 1) {
-        const int rows = std::min(a.max_new * a.group, kFewRows);
-        hipLaunchKernelGGL((paged_attn_join_few_kernel<T, HD>), dim3(a.n_seqs, a.pg.n_kv, (rows + 3) / 4),
+        hipLaunchKernelGGL((paged_attn_join_few_kernel<T, HD>), dim3(a.n_seqs, a.pg.n_kv, (a.few_cap + 3) / 4),
                            dim3(256), 0, st, a);
         SGQ_HIP(hipGetLastError());
     }
@@ -888,13 +942,13 @@ int launch(hipStream_t st, const AttnArgs &a, const Layout &y) {
 
 uint64_t paged_attn_workspace(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, int max_new,
                               int max_kv) {
-    // for rows of either type
-    int s = 1;
+    uint64_t most = 0;  // of both row types
     for (int f16 = 0; f16 < 2; f16++) {
         const Layout y = layout(n_tokens, n_seqs, n_q, n_kv, head_dim, f16, max_new, max_kv);
-        s = std::max(s, std::max(y.few_splits, y.many_splits));
+        most = std::max(most, (y.few_splits > 1 ? y.few_rows * y.few_splits : 0) +
+                                  (y.many_splits > 1 ? y.many_rows * y.many_splits : 0));
     }
-    return s <= 1 ? 0 : (uint64_t)n_tokens * n_q * s * (head_dim + 2) * 4;
+    return most * (head_dim + 2) * 4;
 }
 
 int launch_paged_attn(hipStream_t st, const PagedAttn &p) {
@@ -907,17 +961,28 @@ int launch_paged_attn(hipStream_t st, const PagedAttn &p) {
     a.scale_log2 = p.scale * kLog2e;
     const int reach = p.window > 0 ? (int)std::min<long long>(p.max_kv, (long long)p.window + p.max_new) : p.max_kv;
     const Layout y = layout(p.n_tokens, p.n_seqs, p.n_q, p.pg.n_kv, p.pg.head_dim, p.f16, p.max_new, reach);
-    const uint64_t row_bytes = (uint64_t)p.n_tokens * p.n_q * (p.pg.head_dim + 2) * 4;
-    const uint64_t fit = std::max<uint64_t>(p.workspace ? p.workspace_bytes / row_bytes : 0, 1);
-    a.few = y.few;
-    a.few_splits = (int)std::min<uint64_t>(y.few_splits, fit);
-    a.many_splits = (int)std::min<uint64_t>(y.many_splits, fit);
+    // as many parts as fit into the workspace, the few rows' first
+    const uint64_t part_bytes = (uint64_t)(p.pg.head_dim + 2) * 4;
+    uint64_t room = p.workspace ? p.workspace_bytes / part_bytes : 0;
+    const auto take = [&](uint64_t rows, int splits) {
+        const uint64_t fit = rows ? std::min<uint64_t>(room / rows, splits) : 1;
+        if (fit > 1) room -= rows * fit;
+        return fit > 1 ? (int)fit : 1;
+    };
+    a.few = y.few, a.many_by_token = y.many_by_token;
+    a.few_cap = few_cap(p.max_new, a.group);
+    a.few_splits = take(y.few_rows, y.few_splits);
+    a.many_splits = take(y.many_rows, y.many_splits);
     const int tiles = std::max((int)(((long long)reach + 31) / 32), 1);
     a.few_per = std::max((tiles + a.few_splits - 1) / a.few_splits, 8);
-    a.many_per = std::max((tiles + a.many_splits - 1) / a.many_splits, 8);
-    a.part_slots = std::max(a.few_splits, a.many_splits);
-    a.part = static_cast<float *>(p.workspace);
-    a.part_ml = reinterpret_cast<float2 *>(a.part + (uint64_t)p.n_tokens * p.n_q * a.part_slots * p.pg.head_dim);
+    a.many_per = std::max((tiles + a.many_splits - 1) / a.many_splits, 4);
+    a.many_tiles = y.many_tiles, a.many_whole = a.many_splits > 1 ? y.many_whole : y.many_tiles;
+    const uint64_t few_parts = a.few_splits > 1 ? y.few_rows * a.few_splits : 0;
+    const uint64_t many_parts = a.many_splits > 1 ? y.many_rows * a.many_splits : 0;
+    a.few_part = static_cast<float *>(p.workspace);
+    a.many_part = a.few_part + few_parts * p.pg.head_dim;
+    a.few_ml = reinterpret_cast<float2 *>(a.many_part + many_parts * p.pg.head_dim);
+    a.many_ml = a.few_ml + few_parts;
     switch (p.pg.head_dim * 2 + (p.f16 ? 1 : 0)) {
         case 128 * 2: return launch<float, 128>(st, a, y);
         case 128 * 2 + 1: return launch<_Float16, 128>(st, a, y);
