@@ -53,22 +53,62 @@ __device__ __forceinline__ uint4 regrid(uint4 w, float old, float d, float inv) 
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// Two consecutive activations starting at element 2j.
-__device__ __forceinline__ float2 act_ld2(const float *p, size_t j) {
-    return reinterpret_cast<const float2 *>(p)[j];
-}
-__device__ __forceinline__ float2 act_ld2(const uint16_t *p, size_t j) {
-    const uint32_t w = reinterpret_cast<const uint32_t *>(p)[j];
-    return make_float2(f16_bits_to_f32(w & 0xffffu), f16_bits_to_f32(w >> 16));
+// A block's grid, and four values on it as the bytes of a word.  The low byte of
+// x·(1/scale) + 1.5·2^23 is the rounded quotient, and the residual says whether it may
+// be off: not while it stays below 0.49999 of the scale.  The largest residual goes
+// to `far`; a thread whose unit has one above, or whose grid is so fine that
+// 1/scale may overflow, rounds the unit again the exact way (about one value in 10^5).
+struct Grid {
+    float scale, inv, near_half;
+    uint32_t keep;  // 0 where the scale is 0 or NaN
+    __device__ __forceinline__ explicit Grid(float s)
+        : scale(s), inv(1.f / s), near_half(s < 0x1p-64f ? -1.f : 0.49999f * s), keep(s > 0.f ? ~0u : 0u) {}
+    static __device__ __forceinline__ float raise(float s) { return s < 0x1p-64f ? 0x1p64f : 1.f; }
+    __device__ __forceinline__ bool again(float far) const { return keep && far > near_half; }
+    __device__ __forceinline__ int8_t exact(float x) const {
+        const float up = raise(scale), d = scale * up;
+        return (int8_t)quant_rte(x * up, 0.f, d, 1.f / d);
+    }
+    __device__ __forceinline__ uint32_t quants(float x, float y, float z, float w, float &far) const {
+        constexpr float kMagic = 12582912.f;
+        const float a = fmaf(x, inv, kMagic), b = fmaf(y, inv, kMagic), c = fmaf(z, inv, kMagic), e = fmaf(w, inv, kMagic);
+        far = fmaxf(fmaxf(far, fabsf(fmaf(kMagic - a, scale, x))), fabsf(fmaf(kMagic - b, scale, y)));
+        far = fmaxf(fmaxf(far, fabsf(fmaf(kMagic - c, scale, z))), fabsf(fmaf(kMagic - e, scale, w)));
+        const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x0c0c0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(e), __float_as_uint(c), 0x04000c0cu);
+        return (lo | hi) & keep;
+    }
+};
+
+// Two consecutive activations as they lie, and as numbers.
+template <typename T>
+struct Pair;
+template <>
+struct Pair<float> {
+    typedef float2 Raw;
+    static __device__ __forceinline__ float2 value(Raw x) { return x; }
+};
+template <>
+struct Pair<uint16_t> {
+    typedef uint32_t Raw;
+    static __device__ __forceinline__ float2 value(Raw x) {
+        return make_float2(f16_bits_to_f32(x & 0xffffu), f16_bits_to_f32(x >> 16));
+    }
+};
+
+__device__ __forceinline__ uint32_t most(uint32_t m, float4 x) {  // as bits: NaN > infinity > finite
+    return max(m, max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w))));
 }
 
 // One workgroup writes one run at a time for one head, K (y = 0) or V (y = 1):
 // the runs that begin in its window of `window` rows.  Every wave finds the runs by
-// itself (a load of 64 slots and ballots), the rows are read twice (the second
-// time from the caches): once for the maximum, once to be rounded.
-// K: a thread rounds 8 dims of a row.  V, stored by dim: a thread rounds 2 dims
-// of 16 tokens, so a wave reads whole rows and stores 16 bytes a lane; a dword
-// or byte at a time the stores alone took four times as long as the reads.
+// itself (a load of 64 slots and ballots); the rows are read twice, the second
+// time from the caches: once for the maximum, once to be rounded.  K: a thread
+// rounds 8 dims of a row.  V, stored by dim: a thread rounds 2 dims of 16 tokens,
+// so a wave reads whole rows and stores 16 bytes a lane (a dword or byte at a time
+// the stores alone took four times as long as the reads); only the rows before
+// and behind whole groups of 16 go byte by byte.  Keeping the rows in registers
+// between the two passes halved the waves in flight: 4096 rows 80 us, not 42.
 template <typename T, int HD>
 __global__ __launch_bounds__(kAppThreads) void paged_append_kernel(
     const T *__restrict__ k, uint64_t k_stride, const T *__restrict__ v, uint64_t v_stride,
@@ -132,30 +172,21 @@ __global__ __launch_bounds__(kAppThreads) void paged_append_kernel(
 #pragma unroll 4
         for (int i = tid; i < len * U; i += kAppThreads) {
             const T *x = src + (size_t)(r + i / U) * stride + i % U * 8;
-            const float4 a = act_ld4(x, 0), b = act_ld4(x, 1);
-            // as bits: NaN > infinity > finite
-            amax = max(amax, max(max(abs_bits(a.x), abs_bits(a.y)), max(abs_bits(a.z), abs_bits(a.w))));
-            amax = max(amax, max(max(abs_bits(b.x), abs_bits(b.y)), max(abs_bits(b.z), abs_bits(b.w))));
+            amax = most(most(amax, act_ld4(x, 0)), act_ld4(x, 1));
         }
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, d));
         if (lane == 0) amax_s[tid >> 6] = amax;
         __syncthreads();
         amax = max(max(amax_s[0], amax_s[1]), max(amax_s[2], amax_s[3]));
-        // the run's row at an offset of lo .. hi, -1: none
-        const auto row_at = [&](int off) {
-            return ascend ? (off >= lo && off <= hi ? r + (off - lo) : -1) : row_of[off];
-        };
         const float need = amax >= kInfBits ? __uint_as_float(0x7fc00000u) : __uint_as_float(amax) / 127.f;
         float scale = need;
-        // scale and what it divides both times 2^64 where 1/scale could overflow
-        const auto raise = [](float s) { return s < 0x1p-64f ? 0x1p64f : 1.f; };
-        if (row_at(0) < 0) {
+        if (ascend ? lo > 0 : row_of[0] < 0) {
             if (need != need || old != old) {
                 scale = __uint_as_float(0x7fc00000u);
             } else if (need > old) {
                 uint4 *w = reinterpret_cast<uint4 *>(quants);
-                const float up = raise(need), d = need * up, inv = 1.f / d;
+                const float up = Grid::raise(need), d = need * up, inv = 1.f / d;
                 for (int i = tid; i < (HD << lg) / 16; i += kAppThreads) w[i] = regrid(w[i], old * up, d, inv);
                 __syncthreads();  // the run's quants go over the old ones
             } else {
@@ -163,61 +194,67 @@ __global__ __launch_bounds__(kAppThreads) void paged_append_kernel(
             }
         }
         if (tid == 0) *scale_p = scale;  // every thread has read the old one
-        const bool live = scale > 0.f;   // neither 0 nor NaN
-        const float up = raise(scale), d = scale * up, inv = live ? 1.f / d : 0.f;
-        const auto quant = [&](float x) {
-            return live ? (uint32_t)quant_rte(x * up, 0.f, d, inv) & 0xffu : 0u;
+        const Grid grid(scale);
+        // The offset of row r + i; -1 where another row has its slot.
+        const auto offset_of = [&](int i) {
+            if (ascend) return lo + i;
+            const int off = slots[r + i] & (P - 1);
+            return row_of[off] == r + i ? off : -1;
         };
         if (!is_v) {
-#pragma unroll 4
-            for (int i = tid; i < (hi - lo + 1) * U; i += kAppThreads) {
-                const int off = lo + i / U, c = i % U, row = row_at(off);
-                const T *x = src + (size_t)max(row, r) * stride + c * 8;
+#pragma unroll 2
+            for (int i = tid; i < len * U; i += kAppThreads) {
+                const int off = offset_of(i / U);
+                const T *x = src + (size_t)(r + i / U) * stride + i % U * 8;
                 const float4 a = act_ld4(x, 0), b = act_ld4(x, 1);
-                uint2 o;
-                o.x = quant(a.x) | quant(a.y) << 8 | quant(a.z) << 16 | quant(a.w) << 24;
-                o.y = quant(b.x) | quant(b.y) << 8 | quant(b.z) << 16 | quant(b.w) << 24;
-                if (row >= 0) reinterpret_cast<uint2 *>(quants + (size_t)off * HD)[c] = o;
+                float far = 0.f;
+                const uint2 o = make_uint2(grid.quants(a.x, a.y, a.z, a.w, far), grid.quants(b.x, b.y, b.z, b.w, far));
+                if (off < 0) continue;
+                int8_t *dst = quants + (size_t)off * HD + i % U * 8;
+                *reinterpret_cast<uint2 *>(dst) = o;
+                if (grid.again(far))
+                    for (int e = 0; e < 8; e++) dst[e] = grid.exact(act_ld(x, e));
             }
-        } else {
-            for (int i = tid; i < (hi / 16 - lo / 16 + 1) * (HD / 2); i += kAppThreads) {
-                const int o16 = lo / 16 + i / (HD / 2), c = i % (HD / 2);
-                int8_t *dst = quants + ((size_t)(o16 / 2) * HD + c * 2) * 32 + o16 % 2 * 16;
-                uint32_t w[2][4] = {}, in = 0;
-                const int j0 = max(lo - o16 * 16, 0), j1 = min(hi - o16 * 16, 15);
-                if (j1 - j0 < 2) {  // single tokens, the end of a run: only what is there
-                    for (int j = j0; j <= j1; j++) {
-                        const int row = row_at(o16 * 16 + j);
-                        if (row < 0) continue;
-                        const float2 x = act_ld2(src + (size_t)row * stride, c);
-                        dst[j] = (int8_t)quant(x.x);
-                        dst[32 + j] = (int8_t)quant(x.y);
-                    }
-                    continue;
-                }
-                float2 x[16];
+            continue;
+        }
+        const int g0 = (lo + 15) / 16, groups = ascend ? max((hi + 1) / 16 - g0, 0) : 0;
+        for (int i = tid; i < groups * (HD / 2); i += kAppThreads) {
+            const int o16 = g0 + i / (HD / 2), c = i % (HD / 2);
+            const T *x = src + (size_t)(r + o16 * 16 - lo) * stride + c * 2;
+            typename Pair<T>::Raw raw[16];
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const int row = row_at(o16 * 16 + j);
-                    in |= (row >= 0 ? 1u : 0u) << j;
-                    x[j] = act_ld2(src + (size_t)max(row, r) * stride, c);
-                }
+            for (int j = 0; j < 16; j++) raw[j] = *reinterpret_cast<const typename Pair<T>::Raw *>(x + j * stride);
+            uint32_t w[2][4];
+            float far = 0.f;
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    w[0][j / 4] |= quant(x[j].x) << (j % 4 * 8);
-                    w[1][j / 4] |= quant(x[j].y) << (j % 4 * 8);
-                }
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    if (in == 0xffffu) {
-                        *reinterpret_cast<uint4 *>(dst + e * 32) = make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 16; j++)
-                            if (in >> j & 1) dst[e * 32 + j] = (int8_t)(w[e][j / 4] >> (j % 4 * 8));
-                    }
-                }
+            for (int j = 0; j < 4; j++) {
+                const float2 a = Pair<T>::value(raw[j * 4]), b = Pair<T>::value(raw[j * 4 + 1]);
+                const float2 e = Pair<T>::value(raw[j * 4 + 2]), f = Pair<T>::value(raw[j * 4 + 3]);
+                w[0][j] = grid.quants(a.x, b.x, e.x, f.x, far);
+                w[1][j] = grid.quants(a.y, b.y, e.y, f.y, far);
             }
+            int8_t *dst = quants + ((size_t)(o16 / 2) * HD + c * 2) * 32 + o16 % 2 * 16;
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+            *reinterpret_cast<uint4 *>(dst + 32) = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
+            if (grid.again(far))
+                for (int j = 0; j < 32; j++)
+                    dst[(j >> 4) * 32 + (j & 15)] = grid.exact(act_ld(x + (j & 15) * stride, j >> 4));
+        }
+        const int before_groups = groups ? g0 * 16 - lo : len;
+        for (int i = tid; i < (len - groups * 16) * (HD / 4); i += kAppThreads) {
+            const int e = i / (HD / 4), c = i % (HD / 4), k = e < before_groups ? e : e + groups * 16;
+            const int off = offset_of(k);
+            const T *x = src + (size_t)(r + k) * stride + c * 4;
+            const float4 a = act_ld4(x, 0);
+            float far = 0.f;
+            const uint32_t q = grid.quants(a.x, a.y, a.z, a.w, far);
+            if (off < 0) continue;
+            int8_t *dst = quants + ((size_t)(off / 32) * HD + c * 4) * 32 + off % 32;
+            const bool again = grid.again(far);
+#pragma unroll
+            for (int j = 0; j < 4; j++) dst[j * 32] = (int8_t)(q >> (8 * j));
+            if (again)
+                for (int j = 0; j < 4; j++) dst[j * 32] = grid.exact(act_ld(x, j));
         }
     }
 }
@@ -225,7 +262,7 @@ __global__ __launch_bounds__(kAppThreads) void paged_append_kernel(
 // Slots as values: a half wave reads 4 dims a lane (HD/4 lanes a row) of
 // kGatherRows rows in turn.  V's dword holds 4 tokens of a dim: it is loaded
 // again only when a row leaves it, so consecutive slots read V once.
-constexpr int kGatherRows = 8;
+constexpr int kGatherRows = 4;
 
 template <typename T, int HD>
 __global__ __launch_bounds__(kAppThreads) void paged_gather_kernel(
@@ -276,7 +313,7 @@ int append(hipStream_t st, const PagedPages &pg, const void *k, uint64_t k_strid
            uint64_t v_stride, const int32_t *slots, int n) {
     // few rows: one a workgroup, as they are likely single tokens of many
     // requests; many: runs of up to a page
-    const int window = n <= 512 ? 1 : n <= 2048 ? 4 : 16;
+    const int window = n <= 512 ? 1 : n <= 2048 ? 4 : 63;
     // the heads of a row side by side, as they lie
     const dim3 grid((n + window - 1) / window * pg.n_kv, 2);
     hipLaunchKernelGGL((paged_append_kernel<T, HD>), grid, dim3(kAppThreads), 0, st,
