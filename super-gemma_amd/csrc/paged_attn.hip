@@ -785,66 +785,83 @@ __global__ __launch_bounds__((Many<T, HD>::kThreads), (Many<T, HD>::kWaves / 4))
     }
 }
 
-// Joins the parts of a row, in their order: a wave a row.  Its lanes share out the
-// parts' references and sums, then the dims, four parts' loads in flight.
-template <typename T, int HD>
+// Joins the parts of a row: its W waves take every W-th part, four of them in flight,
+// and are summed in wave order.  The lanes share out the parts' references and
+// sums, then the dims.
+constexpr int kJoinWaves = 4;
+template <typename T, int HD, int W>
 __device__ __forceinline__ void join_row(const AttnArgs &a, const RowTile &rt, int head, int i, int parts,
                                          const float *part, const float2 *part_ml, size_t prow) {
-    const int lane = threadIdx.x & 63, r = rt.row0 + i;
-    const int tok = rt.tok0 + r / a.group, qh = head * a.group + r % a.group;
-    float m = kNoMax, l = 0.f, o[HD / 64];
+    constexpr int ND = HD / 64;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W;
+    const int r = rt.row0 + i, tok = rt.tok0 + r / a.group, qh = head * a.group + r % a.group;
+    float m = kNoMax, l = 0.f, o[ND];
     for (int s = lane; s < parts; s += 64) m = fmaxf(m, part_ml[prow + s].x);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
 #pragma unroll
-    for (int d = 0; d < HD / 64; d++) o[d] = 0.f;
-    for (int b = 0; b < parts; b += 64) {
-        const float2 ml = b + lane < parts ? part_ml[prow + b + lane] : make_float2(kNoMax, 0.f);
-        const float mine = b + lane < parts ? __builtin_amdgcn_exp2f(ml.x - m) : 0.f, ls = ml.y * mine;
-        const int e = min(parts - b, 64);
+    for (int d = 0; d < ND; d++) o[d] = 0.f;
+    for (int b = wave; b < parts; b += 64 * W) {  // lane j: part b + j·W
+        const int mine = b + lane * W;
+        const float2 ml = mine < parts ? part_ml[prow + mine] : make_float2(kNoMax, 0.f);
+        const float f = mine < parts ? __builtin_amdgcn_exp2f(ml.x - m) : 0.f, ls = ml.y * f;
+        const int e = min((parts - b + W - 1) / W, 64);
         for (int s = 0; s < e; s += 4) {
-            float v[4][HD / 64];
+            float v[4][ND];
 #pragma unroll
             for (int k = 0; k < 4; k++)
 #pragma unroll
-                for (int d = 0; d < HD / 64; d++)
-                    v[k][d] = part[(prow + b + min(s + k, e - 1)) * HD + d * 64 + lane];
+                for (int d = 0; d < ND; d++) v[k][d] = part[(prow + b + min(s + k, e - 1) * W) * HD + d * 64 + lane];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 if (s + k >= e) break;
-                const float f = lane_f(mine, s + k);
+                const float fk = lane_f(f, s + k);
                 l += lane_f(ls, s + k);
 #pragma unroll
-                for (int d = 0; d < HD / 64; d++) o[d] = fmaf(v[k][d], f, o[d]);
+                for (int d = 0; d < ND; d++) o[d] = fmaf(v[k][d], fk, o[d]);
             }
         }
     }
-    const float inv = inverse(l);
     T *dst = static_cast<T *>(a.out) + (size_t)tok * a.out_stride + (size_t)qh * HD;
+    if constexpr (W == 1) {
+        const float inv = inverse(l);
 #pragma unroll
-    for (int d = 0; d < HD / 64; d++) dst[d * 64 + lane] = (T)(o[d] * inv);
+        for (int d = 0; d < ND; d++) dst[d * 64 + lane] = (T)(o[d] * inv);
+    } else {
+        static_assert(W == 4, "the sums below");
+        __shared__ float o_s[W][HD], l_s[W];
+#pragma unroll
+        for (int d = 0; d < ND; d++) o_s[wave][d * 64 + lane] = o[d];
+        if (lane == 0) l_s[wave] = l;
+        __syncthreads();
+        const float inv = inverse(l_s[0] + l_s[1] + l_s[2] + l_s[3]);
+        for (int d = threadIdx.x; d < HD; d += W * 64)
+            dst[d] = (T)((o_s[0][d] + o_s[1][d] + o_s[2][d] + o_s[3][d]) * inv);
+    }
 }
 
+// Few rows have many parts: a workgroup a row.
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void paged_attn_join_few_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kJoinWaves * 64) void paged_attn_join_few_kernel(AttnArgs a) {
     RowTile rt;
     if (!few_rows(a, blockIdx.x, &rt)) return;
     const KeySpan ks = key_span(a, rt, a.few_splits, a.few_per);
-    const int i = blockIdx.z * 4 + (threadIdx.x >> 6);
+    const int i = blockIdx.z;
     if (ks.parts > 1 && i < rt.rows)
-        join_row<T, HD>(a, rt, blockIdx.y, i, ks.parts, a.few_part, a.few_ml,
-                        few_row(a, rt, blockIdx.y, i) * a.few_splits);
+        join_row<T, HD, kJoinWaves>(a, rt, blockIdx.y, i, ks.parts, a.few_part, a.few_ml,
+                                    few_row(a, rt, blockIdx.y, i) * a.few_splits);
 }
 
+// Many rows have few parts: a wave a row.
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void paged_attn_join_many_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kJoinWaves * 64) void paged_attn_join_many_kernel(AttnArgs a) {
     RowTile rt;
     if (!many_rows<Many<T, HD>::kRows>(a, a.many_tiles - 1 - a.many_whole - (int)blockIdx.x, &rt)) return;
     const KeySpan ks = key_span(a, rt, a.many_splits, a.many_per);
-    const int i = blockIdx.z * 4 + (threadIdx.x >> 6);
-    if (ks.parts > 1 && i < rt.rows)
-        join_row<T, HD>(a, rt, blockIdx.y, i, ks.parts, a.many_part, a.many_ml,
-                        many_row<Many<T, HD>::kRows>(a, rt, blockIdx.x, blockIdx.y, i) * a.many_splits);
+    if (ks.parts == 1) return;
+    for (int i = blockIdx.z * kJoinWaves + (threadIdx.x >> 6); i < rt.rows; i += gridDim.z * kJoinWaves)
+        join_row<T, HD, 1>(a, rt, blockIdx.y, i, ks.parts, a.many_part, a.many_ml,
+                           many_row<Many<T, HD>::kRows>(a, rt, blockIdx.x, blockIdx.y, i) * a.many_splits);
 }
 
 // How a call is laid out: which kernels run, and into how many parts at most
@@ -927,12 +944,13 @@ int launch(hipStream_t st, const AttnArgs &a, const Layout &y) {
     }
     if (y.many && a.many_splits > 1 && a.many_whole < a.many_tiles) {
         hipLaunchKernelGGL((paged_attn_join_many_kernel<T, HD>),
-                           dim3(a.many_tiles - a.many_whole, a.pg.n_kv, Many<T, HD>::kRows / 4), dim3(256), 0, st, a);
+                           dim3(a.many_tiles - a.many_whole, a.pg.n_kv, Many<T, HD>::kRows / 16),
+                           dim3(kJoinWaves * 64), 0, st, a);
         SGQ_HIP(hipGetLastError());
     }
     if (y.few && a.few_splits > 1) {
-        hipLaunchKernelGGL((paged_attn_join_few_kernel<T, HD>), dim3(a.n_seqs, a.pg.n_kv, (a.few_cap + 3) / 4),
-                           dim3(256), 0, st, a);
+        hipLaunchKernelGGL((paged_attn_join_few_kernel<T, HD>), dim3(a.n_seqs, a.pg.n_kv, a.few_cap),
+                           dim3(kJoinWaves * 64), 0, st, a);
         SGQ_HIP(hipGetLastError());
     }
     return SGQ_OK;

@@ -293,26 +293,29 @@ _ACT = {torch.float32: 0, torch.float16: 1}
 
 def _i32(t, n, dev, name):
     """Device pointer of an int32 tensor of at least n elements."""
-    if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous() or t.numel() < n:
+    if t.dtype != torch.int32 or t.device != dev or t.numel() < n or not t.is_contiguous():
         raise ValidationError(6, f"{name}: contiguous int32 tensor of {n} elements on {dev} expected, "
                                  f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
 def _rows(t, heads, hd, dev, name):
-    """(device pointer, row stride) of packed rows [n, heads, hd] (fp32 or f16),
-    whose rows may lie apart."""
-    if (t.dtype not in _ACT or t.device != dev or t.dim() != 3 or t.shape[1] != heads or
-            t.shape[2] != hd or t.stride(2) != 1 or t.stride(1) != hd):
+    """(device pointer, row stride, rows) of packed rows [n, heads, hd] (fp32 or
+    f16), whose rows may lie apart."""
+    width = heads * hd
+    try:
+        n, h, d = t.shape
+        stride, sh, sd = t.stride()
+    except ValueError:
+        n, h, d, stride, sh, sd = 0, 0, 0, 0, 0, 0
+    if h != heads or d != hd or sd != 1 or sh != hd or t.dtype not in _ACT or t.device != dev:
         raise ValidationError(6, f"{name}: fp32 or f16 rows [n, {heads}, {hd}] on {dev} expected, "
                                  f"got {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
-    stride = t.stride(0)
-    if t.shape[0] < 2:
-        stride = max(stride, heads * hd)  # no second row to reach
-        stride += -stride % 8
-    if stride < heads * hd:
+    if n < 2:
+        stride = width  # no second row to reach
+    elif stride < width:
         raise ValidationError(6, f"{name}: rows overlap (stride {stride})")
-    return t.data_ptr(), stride
+    return t.data_ptr(), stride, n
 
 
 class GpuContext:
@@ -325,6 +328,7 @@ class GpuContext:
         _check(lib().sgq_ctx_create(device, C.byref(h)))
         self._h = h
         self.device = device
+        self._torch_device = torch.device("cuda", device)
         self.set_stream(torch.cuda.current_stream(device))
 
     def __del__(self):
@@ -522,14 +526,11 @@ class GpuContext:
         _check(lib().sgq_add_scaled(self._h, _ptr(a), _ptr(b), _ptr(y), n, s))
 
     # -- paged 8-bit KV cache of a batch of requests --------------------------
-    def _dev(self):
-        return torch.device("cuda", self.device)
-
     def kv_pages_plan(self, cached_lens, new_lens, block_tables, free_list, n_free, n_free_out,
                       kv_lens, cu_tokens, slot_map, missing, page_size: int):
         """Block tables, row offsets and slot map of a step from the requests'
         lengths (sgq_kv_pages_plan).  block_tables [n_seqs, max_pages]; all int32."""
-        dev, n = self._dev(), cached_lens.numel()
+        dev, n = self._torch_device, cached_lens.numel()
         if block_tables.dim() != 2 or block_tables.shape[0] != n:
             raise ValidationError(6, f"block_tables: [{n}, max_pages] expected")
         _check(lib().sgq_kv_pages_plan(
@@ -542,7 +543,7 @@ class GpuContext:
 
     def kv_pages_release(self, done, kv_lens, block_tables, free_list, n_free, page_size: int):
         """Give back the pages of the requests with done != 0 (sgq_kv_pages_release)."""
-        dev, n = self._dev(), kv_lens.numel()
+        dev, n = self._torch_device, kv_lens.numel()
         if block_tables.dim() != 2 or block_tables.shape[0] != n:
             raise ValidationError(6, f"block_tables: [{n}, max_pages] expected")
         _check(lib().sgq_kv_pages_release(
@@ -551,13 +552,13 @@ class GpuContext:
             _i32(free_list, 1, dev, "free_list"), free_list.numel(), _i32(n_free, 1, dev, "n_free")))
 
     def _kv_rows(self, pages: KvPages, k, v, slot_map):
-        dev = self._dev()
+        dev = self._torch_device
         if pages.device != dev:
             raise ValidationError(6, f"pages on {pages.device}, context on {dev}")
-        kp, ks = _rows(k, pages.n_kv, pages.head_dim, dev, "k")
-        vp, vs = _rows(v, pages.n_kv, pages.head_dim, dev, "v")
+        kp, ks, kn = _rows(k, pages.n_kv, pages.head_dim, dev, "k")
+        vp, vs, vn = _rows(v, pages.n_kv, pages.head_dim, dev, "v")
         n = slot_map.numel()
-        if k.dtype != v.dtype or k.shape[0] < n or v.shape[0] < n:
+        if k.dtype != v.dtype or kn < n or vn < n:
             raise ValidationError(6, f"k, v: {n} rows of one type expected")
         return kp, ks, vp, vs, _i32(slot_map, n, dev, "slot_map"), n, _ACT[k.dtype]
 
@@ -583,17 +584,16 @@ class GpuContext:
         (sgq_attn_paged_q8): request s has rows cu_tokens[s]..cu_tokens[s+1]-1, the
         last at position kv_lens[s]-1.  max_kv: about the longest kv_lens (None:
         what the tables hold)."""
-        dev, n = self._dev(), kv_lens.numel()
+        dev, n = self._torch_device, kv_lens.numel()
         if pages.device != dev:
             raise ValidationError(6, f"pages on {pages.device}, context on {dev}")
         if block_tables.dim() != 2 or block_tables.shape[0] != n:
             raise ValidationError(6, f"block_tables: [{n}, max_pages] expected")
         hd, width = pages.head_dim, block_tables.shape[1]
         n_q = q.shape[1] if q.dim() == 3 else 0
-        qp, qs = _rows(q, n_q, hd, dev, "q")
-        op, os_ = _rows(out, n_q, hd, dev, "out")
-        rows = q.shape[0]
-        if out.dtype != q.dtype or out.shape[0] < rows:
+        qp, qs, rows = _rows(q, n_q, hd, dev, "q")
+        op, os_, out_rows = _rows(out, n_q, hd, dev, "out")
+        if out.dtype != q.dtype or out_rows < rows:
             raise ValidationError(6, f"out: {rows} rows of {q.dtype} expected")
         wp, wb = None, 0
         if workspace is not None:

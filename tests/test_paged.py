@@ -739,9 +739,9 @@ def test_tensors_are_checked_before_the_call():
         sgq.KvPages(*good)
     dev = torch.device("cpu")
     rows = z((3, 2, 128))
-    assert sgq._rows(rows, 2, 128, dev, "x") == (rows.data_ptr(), 256)
+    assert sgq._rows(rows, 2, 128, dev, "x") == (rows.data_ptr(), 256, 3)
     assert sgq._rows(z((3, 5, 128))[:, 1:3], 2, 128, dev, "x")[1] == 640
-    assert sgq._rows(z((1, 5, 128)).expand(1, 5, 128)[:, :2], 2, 128, dev, "x")[1] % 8 == 0
+    assert sgq._rows(z((1, 5, 128)).expand(1, 5, 128)[:, :2], 2, 128, dev, "x")[1] == 256
     for bad in (z((3, 2, 64)), z((3, 256)), z((3, 2, 128), dtype=torch.float64), z((3, 128, 2)).transpose(1, 2),
                 z((1, 2, 128)).expand(3, 2, 128), z((3, 2, 256))[..., ::2]):
         with pytest.raises(sgq.ValidationError):
