@@ -364,7 +364,8 @@ int sgq_add_scaled(sgq_ctx *ctx, const float *a, const float *b, float *y, uint6
  *
  * A step is a packed batch: the new tokens of request 0, then of request 1,
  * ..., one row each in q, k, v and out (act: SGQ_ACT_F32 or SGQ_ACT_F16 rows;
- * strides between rows in elements, rows and strides 16-byte aligned).
+ * strides between rows in elements, rows and strides 16-byte aligned).  At most
+ * 2^22 rows, and 2^26 rows x heads.
  * Everything is enqueued on the context's stream, allocates nothing, keeps
  * nothing between calls and can be captured (sgq_graph_begin): lengths,
  * tables and counters are read on the device.  Calls on different streams

@@ -9,6 +9,7 @@ using namespace sgq;
 namespace {
 
 constexpr uint32_t kMaxRows = 1u << 22;  // packed rows of one step
+constexpr uint64_t kMaxRowHeads = 1u << 26;  // rows x heads: every grid below 2^32 threads
 
 bool aligned(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -55,6 +56,13 @@ int check_rows(const char *who, const char *what, const void *p, uint64_t stride
     SGQ_CHECK(stride >= width && stride < (1ull << 32), "%s: %s rows of %llu elements at stride %llu",
               who, what, (unsigned long long)width, (unsigned long long)stride);
     SGQ_CHECK(aligned(p, 16) && stride * es % 16 == 0, "%s: %s rows are not 16-byte aligned", who, what);
+    return SGQ_OK;
+}
+
+int check_count(const char *who, uint32_t n_tokens, uint32_t n_heads) {
+    SGQ_CHECK(n_tokens <= kMaxRows, "%s: n_tokens %u out of range", who, n_tokens);
+    SGQ_CHECK((uint64_t)n_tokens * n_heads <= kMaxRowHeads, "%s: %u rows of %u heads in one step (at most %llu together)",
+              who, n_tokens, n_heads, (unsigned long long)kMaxRowHeads);
     return SGQ_OK;
 }
 
@@ -111,7 +119,7 @@ int sgq_kv_append_paged_q8(sgq_ctx *ctx, const sgq_kv_pages *pages, const void *
         return fail(SGQ_ERR_VALIDATION, "%s: NULL argument", who);
     if (int rc = check_pages(who, pages, &pg)) return rc;
     if (int rc = check_act(who, act)) return rc;
-    SGQ_CHECK(n_tokens <= kMaxRows, "%s: n_tokens %u out of range", who, n_tokens);
+    if (int rc = check_count(who, n_tokens, pages->n_kv_heads)) return rc;
     const uint64_t width = (uint64_t)pg.n_kv * pg.head_dim;
     if (int rc = check_rows(who, "k", k, k_stride, width, act)) return rc;
     if (int rc = check_rows(who, "v", v, v_stride, width, act)) return rc;
@@ -130,7 +138,7 @@ int sgq_kv_gather_paged_q8(sgq_ctx *ctx, const sgq_kv_pages *pages, const int32_
         return fail(SGQ_ERR_VALIDATION, "%s: NULL argument", who);
     if (int rc = check_pages(who, pages, &pg)) return rc;
     if (int rc = check_act(who, act)) return rc;
-    SGQ_CHECK(n_tokens <= kMaxRows, "%s: n_tokens %u out of range", who, n_tokens);
+    if (int rc = check_count(who, n_tokens, pages->n_kv_heads)) return rc;
     const uint64_t width = (uint64_t)pg.n_kv * pg.head_dim;
     if (int rc = check_rows(who, "k", k, k_stride, width, act)) return rc;
     if (int rc = check_rows(who, "v", v, v_stride, width, act)) return rc;
@@ -144,7 +152,8 @@ uint64_t sgq_attn_paged_workspace(const sgq_kv_pages *pages, uint32_t n_seqs, ui
                                   uint32_t n_q_heads, uint32_t max_new, uint32_t max_kv) {
     PagedPages pg;
     if (check_pages("attn_paged_workspace", pages, &pg) || !n_seqs || n_seqs > kPagedMaxSeqs ||
-        !n_tokens || n_tokens > kMaxRows || !n_q_heads || n_q_heads % pg.n_kv)
+        !n_tokens || n_tokens > kMaxRows || !n_q_heads || n_q_heads % pg.n_kv ||
+        n_q_heads / pg.n_kv > 64 || (uint64_t)n_tokens * n_q_heads > kMaxRowHeads)
         return 0;  // the call itself says what is wrong
     return paged_attn_workspace((int)n_tokens, (int)n_seqs, (int)n_q_heads, pg.n_kv, pg.head_dim,
                                 (int)(max_new < kMaxRows ? max_new : kMaxRows),
@@ -164,9 +173,9 @@ int sgq_attn_paged_q8(sgq_ctx *ctx, const sgq_kv_pages *pages, const void *q, ui
     if (int rc = check_pages(who, pages, &a.pg)) return rc;
     if (int rc = check_act(who, act)) return rc;
     if (int rc = check_table(who, n_seqs, pages->page_size, max_pages, pages->n_pages)) return rc;
-    SGQ_CHECK(n_tokens <= kMaxRows, "%s: n_tokens %u out of range", who, n_tokens);
     SGQ_CHECK(n_q_heads >= 1 && n_q_heads % (uint32_t)a.pg.n_kv == 0 && n_q_heads / (uint32_t)a.pg.n_kv <= 64,
               "%s: %u query heads over %d kv heads", who, n_q_heads, a.pg.n_kv);
+    if (int rc = check_count(who, n_tokens, n_q_heads)) return rc;
     SGQ_CHECK(window < (1u << 31), "%s: window %u out of range", who, window);
     SGQ_CHECK(std::isfinite(scale), "%s: scale is not finite", who);
     SGQ_CHECK(aligned(workspace, 16), "%s: workspace is not 16-byte aligned", who);

@@ -52,9 +52,10 @@ struct AttnArgs {
 };
 
 // A tile of query rows of one request and kv head: row r is token r/group of
-// the request's new ones, query head head·group + r%group.
+// the request's new ones, query head head·group + r%group, at position
+// pos0 + r/group.
 struct RowTile {
-    int seq, tok0, new_len, row0, rows, kv_len;
+    int seq, tok0, new_len, row0, rows, kv_len, pos0;
 };
 
 __device__ __forceinline__ int clamped(int v, int lo, int hi) { return min(max(v, lo), hi); }
@@ -70,6 +71,8 @@ __device__ __forceinline__ bool request_rows(const AttnArgs &a, int seq, RowTile
     t->tok0 = c0;
     t->new_len = min(c1 - c0, a.max_new);
     t->kv_len = a.kv_lens[seq];
+    // of the whole request, also where max_new or n_tokens cuts its rows off
+    t->pos0 = t->kv_len - (a.cu[seq + 1] - a.cu[seq]);
     return t->new_len > 0;
 }
 
@@ -109,10 +112,10 @@ __device__ __forceinline__ int key_hi(const AttnArgs &a, int pos, int kv_len) {
 
 // The positions of a row tile's first and last row.
 __device__ __forceinline__ int first_pos(const AttnArgs &a, const RowTile &rt) {
-    return rt.kv_len - rt.new_len + rt.row0 / a.group;
+    return rt.pos0 + rt.row0 / a.group;
 }
 __device__ __forceinline__ int last_pos(const AttnArgs &a, const RowTile &rt) {
-    return rt.kv_len - rt.new_len + (rt.row0 + rt.rows - 1) / a.group;
+    return rt.pos0 + (rt.row0 + rt.rows - 1) / a.group;
 }
 
 // Which 32-key tiles a row tile attends, and into how many parts of `per`
@@ -304,7 +307,7 @@ struct Wave {
 #pragma unroll
                 for (int j = 0; j < NT; j++) {
                     const int row = rt.row0 + min(j * 16 + n, rt.rows - 1);
-                    const int pos = rt.kv_len - rt.new_len + row / a.group;
+                    const int pos = rt.pos0 + row / a.group;
                     const int lo = key_lo(a, pos), hi = min(key_hi(a, pos, rt.kv_len), key_end);
 #pragma unroll
                     for (int k = 0; k < K; k++)
@@ -921,6 +924,8 @@ Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f1
         y.many_whole = full * n_kv / kCus * kCus / n_kv + (y.many_tiles - full);
         if (full * n_kv < kCus) y.many_whole = 0;
         y.many_splits = cut_for((full * n_kv) % kCus, bm * head_dim, max_kv);
+        // mostly empty tiles of very many requests: the grid stays small
+        y.many_splits = std::min(y.many_splits, std::max(1, (1 << 20) / ((y.many_tiles - y.many_whole) * n_kv + 1)));
         if (y.many_splits == 1) y.many_whole = y.many_tiles;
         // with many requests most tiles are empty: then by token
         y.many_rows = (uint64_t)(y.many_tiles - y.many_whole) * n_kv * bm;

@@ -436,6 +436,25 @@ def test_attention_keeps_nan_to_the_rows_that_see_it(ctx, f16, new):
 
 
 @gpu
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("max_new,rows", [(3, 58), (24, 58), (48, 53)])
+def test_attention_of_requests_with_more_rows_than_announced(ctx, f16, max_new, rows):
+    """Rows past max_new or past the buffers are left out; the others keep their positions."""
+    rng = np.random.default_rng(17)
+    page, n_q, n_kv, hd = 32, 4, 2, 128
+    kv, new = [91, 300, 48], [10, 40, 8]
+    host, tables, cu = batch(rng, kv, new, page, n_kv, hd)
+    q = rng.standard_normal((cu[-1], n_q, hd)).astype(np.float16 if f16 else np.float32)
+    got = attend(ctx, to_pages(*host), torch.from_numpy(q[:rows]).cuda(), tables, kv, cu, n_q, max_new=max_new)
+    want, mag, cond, peak = (x[:rows] for x in ref.attention(q, host[0], host[2], host[1], host[3], tables, kv, cu,
+                                                             0, hd ** -0.5, max_new=max_new))
+    live = ~np.isnan(want)
+    assert live.any() and (got[~live] == 7.0).all()
+    bound = ref.attention_bound(want, mag, cond, peak, hd, max(kv), f16)
+    assert (np.abs(got - want) <= bound)[live].all()
+
+
+@gpu
 def test_attention_of_strided_rows_and_a_small_workspace(ctx):
     """q and out as slices of wider rows; a workspace for fewer splits than wanted."""
     rng = np.random.default_rng(3)
@@ -709,6 +728,28 @@ def test_bad_arguments_are_refused():
         v = dict(done=C.c_void_p(0x60000), n=2, page=32, kv=FAKE) | kw
         refused(L.sgq_kv_pages_release(FAKE, v["done"], v["n"], v["page"], v["kv"], FAKE, 4, C.c_void_p(0x70000), 9,
                                        FAKE), text)
+
+
+def test_steps_too_large_for_a_launch_are_refused():
+    """Up to 2^26 (row, head) pairs: below it every grid has fewer than 2^32 threads."""
+    import sgq
+    L = sgq.lib()
+    p = _pages_struct(n_kv=64)
+    pp = C.cast(C.byref(p), C.c_void_p)
+    w, rows = 64 * 128, (1 << 20) + 1
+    refused(L.sgq_kv_append_paged_q8(FAKE, pp, FAKE, w, FAKE, w, 0, FAKE, rows), "heads")
+    refused(L.sgq_kv_gather_paged_q8(FAKE, pp, FAKE, rows, 0, FAKE, w, FAKE, w), "heads")
+    refused(L.sgq_attn_paged_q8(FAKE, pp, FAKE, w, 0, FAKE, 4, FAKE, FAKE, 2, rows, 64, 1, 99, 0, 0.1, FAKE, w,
+                                None, 0), "heads")
+    assert L.sgq_attn_paged_workspace(pp, 2, rows, 64, 1, 99) == 0
+    # the most that is taken, of many requests: no split makes more workgroups than a launch takes
+    for n_kv, n_q, seqs, rows in [(1, 1, 4096, 4096), (100, 100, 4096, 1), (128, 8192, 4096, 4096)]:
+        p = _pages_struct(n_kv=n_kv, n_pages=1 << 20)
+        pp = C.cast(C.byref(p), C.c_void_p)
+        hd_row = (128 + 2) * 4
+        for max_new in (1, 17, 1 << 22):
+            got = L.sgq_attn_paged_workspace(pp, seqs, rows, n_q, max_new, 1 << 25)
+            assert got % hd_row == 0 and got // hd_row < 1 << 31
 
 
 def test_workspace_follows_the_shape():
