@@ -38,15 +38,14 @@ struct AttnArgs {
     uint64_t q_stride, out_stride;
     const int32_t *tables, *kv_lens, *cu;
     // the parts' sums [row][part][hd] and (M, l) [row][part]: rows (request, kv head, row)
-    // of few rows, (cut tile, kv head, row of the tile) or (token, head) of many
+    // of few rows, (cut tile and kv head, row of the tile) of many
     float *few_part, *many_part;
     float2 *few_ml, *many_ml;
     int max_pages, n_seqs, n_tokens, n_q, group, max_new, window;
-    int few_splits, many_splits;  // parts at most, of requests with few and with many rows
-    int few_per, many_per;        // their length in 32-key tiles, if that makes no more of them
-    int many_tiles, many_whole;   // row tiles, and how many of the first (in launch order) stay whole
+    int few_splits, few_per;      // parts at most, of requests with few rows; their 32-key tiles, if
+                                  // that makes no more of them
     int few_cap;                  // rows a request of few has at most
-    bool many_by_token;           // whichever is fewer rows
+    int many_tiles, many_room;    // row tiles at most; parts that the workspace holds
     bool few;                     // requests with few rows go to their own kernel
     float scale_log2;
 };
@@ -84,21 +83,103 @@ __device__ __forceinline__ bool few_rows(const AttnArgs &a, int seq, RowTile *t)
     return true;
 }
 
-// Tile `id` of BM rows.  Request s owns the ids from floor(cu_s·group/BM) + s
-// on, which is room for its ceil(new·group/BM) tiles; ids left over are empty.
+// 256 requests' tiles of BM rows, four requests a lane.
 template <int BM>
-__device__ __forceinline__ bool many_rows(const AttnArgs &a, int id, RowTile *t) {
-    int lo = 0, hi = a.n_seqs;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        const long long c = clamped(a.cu[mid], 0, a.n_tokens);
-        if (c * a.group / BM + mid <= id) lo = mid;
-        else hi = mid;
+struct ManyScan {
+    int n[4], end;  // of each; of all up to this lane's last
+    int reach;      // keys that a row tile attends at most
+    __device__ __forceinline__ void load(const AttnArgs &a, int b) {
+        const int lane = threadIdx.x & 63;
+        int cu[5], kv[4];
+#pragma unroll
+        for (int k = 0; k < 5; k++) cu[k] = clamped(a.cu[min(b + lane * 4 + k, a.n_seqs)], 0, a.n_tokens);
+#pragma unroll
+        for (int k = 0; k < 4; k++) kv[k] = a.kv_lens[min(b + lane * 4 + k, a.n_seqs - 1)];
+        end = reach = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int rows = min(max(cu[k + 1] - cu[k], 0), a.max_new) * a.group;
+            n[k] = a.few && rows <= kFewRows ? 0 : (rows + BM - 1) / BM;
+            end += n[k];
+            const int wide = kv[k] - (BM - 1) / a.group;
+            if (n[k]) reach = max(reach, a.window > 0 && wide > a.window ? kv[k] - wide + a.window : kv[k]);
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(end, d);
+            end += lane >= d ? o : 0;
+        }
     }
-    if (!request_rows(a, lo, t) || (a.few && t->new_len * a.group <= kFewRows)) return false;
-    t->row0 = (id - (int)((long long)t->tok0 * a.group / BM) - lo) * BM;
-    t->rows = min(t->new_len * a.group - t->row0, BM);
-    return t->row0 >= 0 && t->rows > 0;
+};
+
+// How a call's row tiles are launched: the last ones, which attend most keys, first.
+// As many as fill the GPU a whole number of times (a workgroup a CU) stay whole; the
+// keys of what is left are cut into `splits` parts of `per` 32-key tiles.  Every
+// wave works it out from the lengths (a lane a number of parts): the host knows
+// bounds only.
+struct ManyPlan {
+    int tiles, whole, splits, per;
+};
+constexpr int kCus = 256;
+__host__ __device__ __forceinline__ int whole_tiles(int tiles, int n_kv) { return tiles * n_kv / kCus * kCus / n_kv; }
+
+// The microseconds of `units` workgroups of `area` rows x dims with p parts of `per`
+// tiles: a round costs its tiles, 1.3 each (1.1 to 2.1 measured), and four for its
+// start; joining moves the parts twice, at 4 TB/s.
+__host__ __device__ __forceinline__ float parts_cost(int units, int p, int per, int area) {
+    return 1.3f * ((units * p + kCus - 1) / kCus) * (per + 4) + (p > 1 ? 5.f + 2e-6f * area * units * p : 0.f);
+}
+
+template <int BM, int HD>
+__device__ __forceinline__ ManyPlan many_plan(const AttnArgs &a, ManyScan<BM> &scan) {
+    ManyPlan m;
+    m.tiles = 0;
+    int reach = 0;
+    for (int b = 0; b < a.n_seqs; b += 256) {
+        scan.load(a, b);
+        m.tiles += __builtin_amdgcn_readlane(scan.end, 63);
+        reach = max(reach, scan.reach);
+    }
+    m.tiles = clamped(m.tiles, 0, a.many_tiles);
+    m.whole = m.tiles, m.splits = 1, m.per = INT32_MAX;
+    const int whole = whole_tiles(m.tiles, a.pg.n_kv), units = (m.tiles - whole) * a.pg.n_kv;
+    if (a.many_room < 2 * units || units == 0) return m;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) reach = max(reach, __shfl_xor(reach, d));
+    const int p = (threadIdx.x & 63) + 1, keys = min(reach, a.max_pages << a.pg.page_log2) / 32 + 1;
+    const int per = (keys + p - 1) / p;
+    float us = parts_cost(units, p, per, BM * HD);
+    if (p > 1 && (per < 4 || units * p > a.many_room)) us = INFINITY;
+    float least = us;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) least = fminf(least, __shfl_xor(least, d));
+    const int best = __builtin_ctzll(__ballot(us == least));
+    if (best == 0) return m;
+    m.whole = whole, m.splits = best + 1, m.per = __builtin_amdgcn_readlane(per, best);
+    return m;
+}
+
+// Tile `id` of the plan that `scan` was made for.
+template <int BM>
+__device__ __forceinline__ bool many_rows(const AttnArgs &a, ManyScan<BM> &scan, int id, RowTile *t) {
+    int before = 0;
+    for (int b = 0; b < a.n_seqs; b += 256) {
+        if (a.n_seqs > 256) scan.load(a, b);
+        if (const uint64_t past = __ballot(before + scan.end > id)) {
+            int k = 0, first = before + scan.end - (scan.n[0] + scan.n[1] + scan.n[2] + scan.n[3]);
+#pragma unroll
+            for (int i = 0; i < 3; i++)
+                if (k == i && first + scan.n[i] <= id) first += scan.n[i], k++;
+            const int owner = __builtin_ctzll(past);
+            first = __builtin_amdgcn_readlane(first, owner);
+            if (!request_rows(a, b + owner * 4 + __builtin_amdgcn_readlane(k, owner), t)) return false;
+            t->row0 = (id - first) * BM;
+            t->rows = min(t->new_len * a.group - t->row0, BM);
+            return t->row0 >= 0 && t->rows > 0;
+        }
+        before += __builtin_amdgcn_readlane(scan.end, 63);
+    }
+    return false;
 }
 
 // Keys [lo, hi) of the query at position pos.
@@ -212,6 +293,7 @@ template <typename T, int HD, int NT>
 struct Wave {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int NC = HD / 64, ND = HD / 16;
+    h8 (*ql_s)[64] = nullptr;
     h8 qa[NT][NC][2], ql[F32 ? NT : 1][F32 ? NC : 1][2];
     // x = s·(row_scale·ks) + row_raise·ks: f16 rows meet K raised by 128, and the
     // second term takes 128·Σq away.  Its rounding is 2^-24 of numbers some
@@ -404,6 +486,10 @@ struct Wave {
         // One tile.  Its V and then the next tile's K are on their way while it is
         // worked on; the last tile has a copy of this code without that K, as a
         // load under a condition would be waited for at once.
+        const auto low = [&](int j, int c, int e) {
+            if constexpr (F32 && HD == 512) return ql_s[c * 2 + e][lane];
+            else return ql[j][c][e];
+        };
         const auto tile = [&](int i, int t, auto more) {
             float sc[1][3];
             pages.scales(i % 64, sc[0]);
@@ -423,13 +509,13 @@ struct Wave {
                     for (int j = 0; j < NT; j++) {
                         s[j][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qa[j][c][0], s[j][h], 0, 0, 0);
                         if constexpr (F32)
-                            s[j][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[j][c][0], s[j][h], 0, 0, 0);
+                            s[j][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, low(j, c, 0), s[j][h], 0, 0, 0);
                     }
 #pragma unroll
                     for (int j = 0; j < NT; j++) {
                         s[j][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qa[j][c][1], s[j][h], 0, 0, 0);
                         if constexpr (F32)
-                            s[j][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[j][c][1], s[j][h], 0, 0, 0);
+                            s[j][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, low(j, c, 1), s[j][h], 0, 0, 0);
                     }
                 }
             if constexpr (decltype(more)::value) {
@@ -469,14 +555,6 @@ __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f 
 __device__ __forceinline__ size_t few_row(const AttnArgs &a, const RowTile &rt, int head, int i) {
     return ((size_t)rt.seq * a.pg.n_kv + head) * a.few_cap + i;
 }
-template <int BM>
-__device__ __forceinline__ size_t many_row(const AttnArgs &a, const RowTile &rt, int cut_tile, int head, int i) {
-    if (a.many_by_token) {
-        const int r = rt.row0 + i;
-        return (size_t)(rt.tok0 + r / a.group) * a.n_q + head * a.group + r % a.group;
-    }
-    return ((size_t)cut_tile * a.pg.n_kv + head) * BM + i;
-}
 
 // Few rows: one request and kv head against one part of the keys, the tiles dealt
 // to 4 waves in turn and their sums joined in LDS in wave order.
@@ -498,6 +576,14 @@ __global__ __launch_bounds__(kFewWaves * 64, HD == 128 ? 3 : HD == 256 ? 2 : 1) 
     const int t0 = ks.t0 + split * ks.per, t1 = min(t0 + ks.per, ks.t1);
     Wave<T, HD, 1> w;
     w.template load_q<true>(a, rt, head, n, g);
+    if constexpr (Wave<T, HD, 1>::F32 && HD == 512) {
+        __shared__ h8 ql_s[NC * 2][64];
+        if (wave == 0)
+#pragma unroll
+            for (int c = 0; c < NC; c++) ql_s[c * 2][lane] = w.ql[0][c][0], ql_s[c * 2 + 1][lane] = w.ql[0][c][1];
+        __syncthreads();
+        w.ql_s = ql_s;
+    }
     w.template attend<true>(a, rt, head, t0 + wave, t1, kFewWaves, lane);
     if (g == 0) {
         ml_s[wave][0][n] = w.M[0];
@@ -584,16 +670,18 @@ __global__ __launch_bounds__((Many<T, HD>::kThreads), (Many<T, HD>::kWaves / 4))
     // in a scalar register: what follows from it, barriers among it, branches for the
     // whole wave
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // XCD = id % 8 takes heads congruent to it, so its L2 holds their pages; the
-    // last tiles, which attend most keys, go first
-    const int n_whole = a.many_whole * a.pg.n_kv, n_cut = (a.many_tiles - a.many_whole) * a.pg.n_kv;
+    // XCD = id % 8 takes heads congruent to it, so its L2 holds their pages
+    ManyScan<C::kRows> scan;
+    const ManyPlan plan = many_plan<C::kRows, HD>(a, scan);
+    const int n_whole = plan.whole * a.pg.n_kv, n_cut = (plan.tiles - plan.whole) * a.pg.n_kv;
     const bool whole = (int)blockIdx.x < n_whole;
-    const int y = whole ? blockIdx.x : (blockIdx.x - n_whole) % n_cut;
+    if (!whole && (int)blockIdx.x - n_whole >= n_cut * plan.splits) return;
+    const int unit = whole ? blockIdx.x : (blockIdx.x - n_whole) % n_cut;
     const int split = whole ? 0 : (blockIdx.x - n_whole) / n_cut;
-    const int head = y % a.pg.n_kv, rank = y / a.pg.n_kv + (whole ? 0 : a.many_whole);
+    const int head = unit % a.pg.n_kv, rank = unit / a.pg.n_kv + (whole ? 0 : plan.whole);
     RowTile rt;
-    if (!many_rows<C::kRows>(a, a.many_tiles - 1 - rank, &rt)) return;
-    const KeySpan ks = key_span(a, rt, whole ? 1 : a.many_splits, a.many_per);
+    if (!many_rows(a, scan, plan.tiles - 1 - rank, &rt)) return;
+    const KeySpan ks = key_span(a, rt, whole ? 1 : plan.splits, whole ? 1 : plan.per);
     if (split >= ks.parts) return;
     const int t0 = ks.t0 + split * ks.per, t1 = min(t0 + ks.per, ks.t1);
 
@@ -779,8 +867,7 @@ __global__ __launch_bounds__((Many<T, HD>::kThreads), (Many<T, HD>::kWaves / 4))
 #pragma unroll
             for (int d = 0; d < HD / 16; d++) store4(dst + d * 16, scaled(w.acc[j][d], inv));
         } else {
-            const size_t prow =
-                many_row<C::kRows>(a, rt, rank - a.many_whole, head, row - rt.row0) * a.many_splits + split;
+            const size_t prow = ((size_t)unit * C::kRows + row - rt.row0) * plan.splits + split;
 #pragma unroll
             for (int d = 0; d < HD / 16; d++) store4(a.many_part + prow * HD + d * 16 + g * 4, scaled(w.acc[j][d], 1.f));
             if (g == 0) a.many_ml[prow] = make_float2(w.M[j], w.l[j]);
@@ -843,39 +930,53 @@ __device__ __forceinline__ void join_row(const AttnArgs &a, const RowTile &rt, i
     }
 }
 
-// Few rows have many parts: a workgroup a row.
-template <typename T, int HD>
-__global__ __launch_bounds__(kJoinWaves * 64) void paged_attn_join_few_kernel(AttnArgs a) {
+// Many rows have few parts: the waves of n_many workgroups take them in turn.  Few
+// rows have many: a workgroup a row of a single token.
+template <typename T, int HD, bool MANY>
+__global__ __launch_bounds__(kJoinWaves * 64) void paged_attn_join_kernel(AttnArgs a, int n_many) {
     RowTile rt;
-    if (!few_rows(a, blockIdx.x, &rt)) return;
-    const KeySpan ks = key_span(a, rt, a.few_splits, a.few_per);
-    const int i = blockIdx.z;
-    if (ks.parts > 1 && i < rt.rows)
-        join_row<T, HD, kJoinWaves>(a, rt, blockIdx.y, i, ks.parts, a.few_part, a.few_ml,
-                                    few_row(a, rt, blockIdx.y, i) * a.few_splits);
-}
-
-// Many rows have few parts: a wave a row.
-template <typename T, int HD>
-__global__ __launch_bounds__(kJoinWaves * 64) void paged_attn_join_many_kernel(AttnArgs a) {
-    RowTile rt;
-    if (!many_rows<Many<T, HD>::kRows>(a, a.many_tiles - 1 - a.many_whole - (int)blockIdx.x, &rt)) return;
-    const KeySpan ks = key_span(a, rt, a.many_splits, a.many_per);
-    if (ks.parts == 1) return;
-    for (int i = blockIdx.z * kJoinWaves + (threadIdx.x >> 6); i < rt.rows; i += gridDim.z * kJoinWaves)
-        join_row<T, HD, 1>(a, rt, blockIdx.y, i, ks.parts, a.many_part, a.many_ml,
-                           many_row<Many<T, HD>::kRows>(a, rt, blockIdx.x, blockIdx.y, i) * a.many_splits);
+    if (!MANY || (int)blockIdx.x >= n_many) {
+        const int each = MANY ? min(a.group, a.few_cap) : gridDim.z, id = blockIdx.x - n_many;
+        const int head = MANY ? id / each % a.pg.n_kv : blockIdx.y, seq = MANY ? id / each / a.pg.n_kv : blockIdx.x;
+        int i = MANY ? id % each : blockIdx.z;
+        if (!few_rows(a, seq, &rt)) return;
+        const KeySpan ks = key_span(a, rt, a.few_splits, a.few_per);
+        if (ks.parts == 1 || i >= rt.rows) return;
+        for (;;) {
+            join_row<T, HD, kJoinWaves>(a, rt, head, i, ks.parts, a.few_part, a.few_ml,
+                                        few_row(a, rt, head, i) * a.few_splits);
+            i += each;
+            if (i >= rt.rows) break;
+            __syncthreads();  // its LDS is read
+        }
+        return;
+    }
+    constexpr int BM = Many<T, HD>::kRows;
+    ManyScan<BM> scan;
+    const ManyPlan plan = many_plan<BM, HD>(a, scan);
+    const int units = (plan.tiles - plan.whole) * a.pg.n_kv;
+    const int first = blockIdx.x * kJoinWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int w = first; w < units * BM; w += n_many * kJoinWaves) {
+        const int unit = w / BM, i = w % BM, head = unit % a.pg.n_kv;
+        if (!many_rows(a, scan, plan.tiles - 1 - plan.whole - unit / a.pg.n_kv, &rt) || i >= rt.rows) continue;
+        const KeySpan ks = key_span(a, rt, plan.splits, plan.per);
+        if (ks.parts > 1)
+            join_row<T, HD, 1>(a, rt, head, i, ks.parts, a.many_part, a.many_ml, (size_t)w * plan.splits);
+    }
 }
 
 // How a call is laid out: which kernels run, and into how many parts at most
 // they cut the keys of a row.
 constexpr int kFewWgs = 1024;
-constexpr int kCus = 256;
 int few_cap(int max_new, int group) { return (int)std::min<long long>((long long)max_new * group, kFewRows); }
+// Parts of many rows, together: three rounds.
+constexpr int kManyParts = 3 * kCus;
+constexpr int kJoinWgs = 8 * kCus;  // of many rows: as many as fit
 struct Layout {
-    bool few, many, many_by_token;
-    int few_splits, many_splits, many_tiles, many_whole;
-    uint64_t few_rows, many_rows;  // that may be cut
+    bool few, many;
+    int few_splits, many_tiles, many_parts;
+    uint64_t few_rows;  // that may be cut
+    int many_bm;        // rows of a tile
 };
 
 // Parts of 256 keys or more, so many that `units` workgroups of one part each
@@ -886,22 +987,6 @@ int splits_for(long long units, long long wanted, int max_kv) {
     return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
 }
 
-// Parts for `units` workgroups (below a round of the GPU, one a CU, or what is left
-// after whole rounds) of row tiles with `area` rows x dims.  A round costs its
-// tiles of 32 keys, 1.3 us each (1.1 to 2.1 measured), and four for its start;
-// joining p parts moves them twice, at 4 TB/s.
-int cut_for(int units, int area, int max_kv) {
-    const int tiles = (int)(((long long)max_kv + 31) / 32);
-    int best = 1;
-    double least = 0;
-    for (int p = 1; p <= 64 && (p == 1 || tiles / p >= 4); p++) {
-        const double rounds = (units * p + kCus - 1) / kCus;
-        const double us = 1.3 * rounds * ((tiles + p - 1) / p + 4) + (p > 1 ? 5 + 2e-6 * area * units * p : 0);
-        if (p == 1 || us < least) best = p, least = us;
-    }
-    return best;
-}
-
 Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f16, int max_new, int max_kv) {
     const int group = n_q / n_kv;
     Layout y{};
@@ -909,28 +994,31 @@ Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f1
     // needs one kernel
     y.many = (long long)max_new * group > kFewRows;
     y.few = !y.many || n_seqs > 1;
-    y.few_splits = y.many_splits = 1;
+    y.few_splits = 1;
+    y.many_bm = 1;
     if (y.few) {
         y.few_splits = splits_for((long long)n_seqs * n_kv, kFewWgs, max_kv);
         y.few_rows = (uint64_t)n_seqs * n_kv * few_cap(max_new, group);
     }
     if (y.many) {
-        const int bm = head_dim == 128 ? (f16 ? Many<_Float16, 128>::kRows : Many<float, 128>::kRows)
-                       : head_dim == 256 ? (f16 ? Many<_Float16, 256>::kRows : Many<float, 256>::kRows)
-                                         : (f16 ? Many<_Float16, 512>::kRows : Many<float, 512>::kRows);
-        y.many_tiles = (int)((long long)n_tokens * group / bm) + n_seqs;
-        // The room for more tiles than one request with all rows has is mostly empty.
-        const int full = (int)((long long)n_tokens * group / bm) + 1;
-        y.many_whole = full * n_kv / kCus * kCus / n_kv + (y.many_tiles - full);
-        if (full * n_kv < kCus) y.many_whole = 0;
-        y.many_splits = cut_for((full * n_kv) % kCus, bm * head_dim, max_kv);
-        // mostly empty tiles of very many requests: the grid stays small
-        y.many_splits = std::min(y.many_splits, std::max(1, (1 << 20) / ((y.many_tiles - y.many_whole) * n_kv + 1)));
-        if (y.many_splits == 1) y.many_whole = y.many_tiles;
-        // with many requests most tiles are empty: then by token
-        y.many_rows = (uint64_t)(y.many_tiles - y.many_whole) * n_kv * bm;
-        y.many_by_token = y.many_rows > (uint64_t)n_tokens * n_q;
-        if (y.many_by_token) y.many_rows = (uint64_t)n_tokens * n_q;
+        y.many_bm = head_dim == 128   ? (f16 ? Many<_Float16, 128>::kRows : Many<float, 128>::kRows)
+                    : head_dim == 256 ? (f16 ? Many<_Float16, 256>::kRows : Many<float, 256>::kRows)
+                                      : (f16 ? Many<_Float16, 512>::kRows : Many<float, 512>::kRows);
+        // a request with many rows has more than kFewRows, and a last tile that is not full
+        const int last = y.few ? (int)std::min<long long>(n_seqs, (long long)n_tokens * group / (kFewRows + 1)) : 1;
+        y.many_tiles = (int)((long long)n_tokens * group / y.many_bm) + std::max(last, 1);
+        y.many_parts = std::min<long long>(kManyParts, 64ll * y.many_tiles * n_kv);
+        if (n_seqs == 1) {  // its rows are known, and so are its parts
+            const int tiles = (int)(((long long)n_tokens * group + y.many_bm - 1) / y.many_bm);
+            const int units = (tiles - whole_tiles(tiles, n_kv)) * n_kv, keys = max_kv / 32 + 1;
+            float least = parts_cost(units, 1, keys, y.many_bm * head_dim);
+            int best = 0;
+            for (int p = 2; p <= 64 && keys / p >= 4 && units * p <= y.many_parts; p++) {
+                const float us = parts_cost(units, p, (keys + p - 1) / p, y.many_bm * head_dim);
+                if (us < least) least = us, best = p;
+            }
+            y.many_parts = units * best;
+        }
     }
     return y;
 }
@@ -938,7 +1026,7 @@ Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f1
 template <typename T, int HD>
 int launch(hipStream_t st, const AttnArgs &a, const Layout &y) {
     if (y.many) {
-        const int wgs = (a.many_whole + (a.many_tiles - a.many_whole) * a.many_splits) * a.pg.n_kv;
+        const int wgs = a.many_tiles * a.pg.n_kv + a.many_room;
         hipLaunchKernelGGL((paged_attn_many_kernel<T, HD>), dim3(wgs), dim3(Many<T, HD>::kThreads), 0, st, a);
         SGQ_HIP(hipGetLastError());
     }
@@ -947,15 +1035,15 @@ int launch(hipStream_t st, const AttnArgs &a, const Layout &y) {
                            dim3(kFewWaves * 64), 0, st, a);
         SGQ_HIP(hipGetLastError());
     }
-    if (y.many && a.many_splits > 1 && a.many_whole < a.many_tiles) {
-        hipLaunchKernelGGL((paged_attn_join_many_kernel<T, HD>),
-                           dim3(a.many_tiles - a.many_whole, a.pg.n_kv, Many<T, HD>::kRows / 16),
-                           dim3(kJoinWaves * 64), 0, st, a);
+    const int each = std::min(a.group, a.few_cap), n_few = a.few_splits > 1 ? a.n_seqs * a.pg.n_kv * each : 0;
+    if (a.many_room > 1) {
+        const long long units = std::min<long long>(a.many_room / 2, (long long)a.many_tiles * a.pg.n_kv);
+        const int n_many = (int)std::min<long long>(kJoinWgs, units * Many<T, HD>::kRows / kJoinWaves);
+        hipLaunchKernelGGL((paged_attn_join_kernel<T, HD, true>), dim3(n_many + n_few), dim3(kJoinWaves * 64), 0, st, a,
+                           n_many);
         SGQ_HIP(hipGetLastError());
-    }
-    if (y.few && a.few_splits > 1) {
-        hipLaunchKernelGGL((paged_attn_join_few_kernel<T, HD>), dim3(a.n_seqs, a.pg.n_kv, a.few_cap),
-                           dim3(kJoinWaves * 64), 0, st, a);
+    } else if (n_few) {
+        hipLaunchKernelGGL((paged_attn_join_kernel<T, HD, false>), dim3(a.n_seqs, a.pg.n_kv, each), dim3(kJoinWaves * 64), 0, st, a, 0);
         SGQ_HIP(hipGetLastError());
     }
     return SGQ_OK;
@@ -969,7 +1057,7 @@ uint64_t paged_attn_workspace(int n_tokens, int n_seqs, int n_q, int n_kv, int h
     for (int f16 = 0; f16 < 2; f16++) {
         const Layout y = layout(n_tokens, n_seqs, n_q, n_kv, head_dim, f16, max_new, max_kv);
         most = std::max(most, (y.few_splits > 1 ? y.few_rows * y.few_splits : 0) +
-                                  (y.many_splits > 1 ? y.many_rows * y.many_splits : 0));
+                                  (uint64_t)y.many_parts * y.many_bm);
     }
     return most * (head_dim + 2) * 4;
 }
@@ -987,21 +1075,19 @@ int launch_paged_attn(hipStream_t st, const PagedAttn &p) {
     // as many parts as fit into the workspace, the few rows' first
     const uint64_t part_bytes = (uint64_t)(p.pg.head_dim + 2) * 4;
     uint64_t room = p.workspace ? p.workspace_bytes / part_bytes : 0;
-    const auto take = [&](uint64_t rows, int splits) {
-        const uint64_t fit = rows ? std::min<uint64_t>(room / rows, splits) : 1;
-        if (fit > 1) room -= rows * fit;
-        return fit > 1 ? (int)fit : 1;
-    };
-    a.few = y.few, a.many_by_token = y.many_by_token;
-    a.few_cap = few_cap(p.max_new, a.group);
-    a.few_splits = take(y.few_rows, y.few_splits);
-    a.many_splits = take(y.many_rows, y.many_splits);
+    if (y.few_splits > 1 && room >= 2 * y.few_rows) {
+        a.few_splits = (int)std::min<uint64_t>(room / y.few_rows, y.few_splits);
+        room -= y.few_rows * a.few_splits;
+    } else {
+        a.few_splits = 1;
+    }
     const int tiles = std::max((int)(((long long)reach + 31) / 32), 1);
     a.few_per = std::max((tiles + a.few_splits - 1) / a.few_splits, 8);
-    a.many_per = std::max((tiles + a.many_splits - 1) / a.many_splits, 4);
-    a.many_tiles = y.many_tiles, a.many_whole = a.many_splits > 1 ? y.many_whole : y.many_tiles;
+    a.few = y.few, a.few_cap = few_cap(p.max_new, a.group);
+    a.many_tiles = y.many_tiles;
+    a.many_room = (int)std::min<uint64_t>(room / y.many_bm, y.many_parts);
     const uint64_t few_parts = a.few_splits > 1 ? y.few_rows * a.few_splits : 0;
-    const uint64_t many_parts = a.many_splits > 1 ? y.many_rows * a.many_splits : 0;
+    const uint64_t many_parts = (uint64_t)a.many_room * y.many_bm;
     a.few_part = static_cast<float *>(p.workspace);
     a.many_part = a.few_part + few_parts * p.pg.head_dim;
     a.few_ml = reinterpret_cast<float2 *>(a.many_part + many_parts * p.pg.head_dim);
