@@ -293,8 +293,8 @@ template <typename T, int HD, int NT>
 struct Wave {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int NC = HD / 64, ND = HD / 16;
-    h8 (*ql_s)[64] = nullptr;
     h8 qa[NT][NC][2], ql[F32 ? NT : 1][F32 ? NC : 1][2];
+    h8 (*ql_s)[64];  // fp32 rows of 512 dims, few: ql [fragment][lane] in LDS
     // x = s·(row_scale·ks) + row_raise·ks: f16 rows meet K raised by 128, and the
     // second term takes 128·Σq away.  Its rounding is 2^-24 of numbers some
     // four times the scores: far below an f16 weight's, not below an fp32 one's.
@@ -577,6 +577,9 @@ __global__ __launch_bounds__(kFewWaves * 64, HD == 128 ? 3 : HD == 256 ? 2 : 1) 
     Wave<T, HD, 1> w;
     w.template load_q<true>(a, rt, head, n, g);
     if constexpr (Wave<T, HD, 1>::F32 && HD == 512) {
+        // both halves of q, the accumulator and a tile on its way are more registers than
+        // a wave has (84 spilled): the waves' common low half from LDS, 174 -> 119 us
+        // for 16 requests of 8192 keys
         __shared__ h8 ql_s[NC * 2][64];
         if (wave == 0)
 #pragma unroll
@@ -967,7 +970,6 @@ __global__ __launch_bounds__(kJoinWaves * 64) void paged_attn_join_kernel(AttnAr
 
 // How a call is laid out: which kernels run, and into how many parts at most
 // they cut the keys of a row.
-constexpr int kFewWgs = 1024;
 int few_cap(int max_new, int group) { return (int)std::min<long long>((long long)max_new * group, kFewRows); }
 // Parts of many rows, together: three rounds.
 constexpr int kManyParts = 3 * kCus;
@@ -979,12 +981,17 @@ struct Layout {
     int many_bm;        // rows of a tile
 };
 
-// Parts of 256 keys or more, so many that `units` workgroups of one part each
-// become `wanted` of them.
-int splits_for(long long units, long long wanted, int max_kv) {
-    const long long by_fill = (wanted + units - 1) / units, by_keys = ((long long)max_kv + 255) / 256;
-    const long long s = by_fill < by_keys ? by_fill : by_keys;
-    return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+// Parts of 256 keys or more of a request with few rows.  One workgroup a CU when that
+// comes out even: each then reads long runs, and one a CU draws the whole
+// bandwidth (one request of 32768 keys, 16 heads of 128, fp32: 29 us with 256 of them, 33
+// with 1024; 16 of 4096: 39 and 44).  Otherwise four a CU, as requests differ in
+// length and what is left over weighs less (6 requests of 6000: 41 and 28);
+// at 512 dims a CU has room for one, and more only queue (16 fp32 of 8192: 90 and 119).
+int splits_for(int units, int head_dim, int max_kv) {
+    const bool even = kCus % units == 0 || units % kCus == 0;
+    const int by_fill = ((even || head_dim == 512 ? kCus : 4 * kCus) + units - 1) / units;
+    const int by_keys = (int)(((long long)max_kv + 255) / 256);
+    return std::clamp(by_fill, 1, std::max(by_keys, 1));
 }
 
 Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f16, int max_new, int max_kv) {
@@ -997,7 +1004,7 @@ Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f1
     y.few_splits = 1;
     y.many_bm = 1;
     if (y.few) {
-        y.few_splits = splits_for((long long)n_seqs * n_kv, kFewWgs, max_kv);
+        y.few_splits = splits_for(n_seqs * n_kv, head_dim, max_kv);
         y.few_rows = (uint64_t)n_seqs * n_kv * few_cap(max_new, group);
     }
     if (y.many) {
