@@ -614,6 +614,96 @@ def test_a_captured_decode_step_replays_with_growing_lengths():
 
 
 @gpu
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("n", [255, 300, 700])
+def test_attention_of_many_requests(ctx, f16, n):
+    """Single tokens, chunks and empty requests in batches past one scan of the
+    lengths; a few requests are long enough to be cut."""
+    rng = np.random.default_rng(n)
+    new = rng.choice([0, 1, 1, 1, 2, 20, 41], n)
+    kv = new + rng.integers(0, 70, n)
+    for s in (0, n // 2, n - 1):
+        new[s], kv[s] = (1, 45, 150)[s * 2 // n], 700
+    check_attention(ctx, n, list(kv), list(new), 32, 2, 1, 128, f16, rows=int(new.sum()) + 3)
+
+
+@gpu
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("hd,n_q,n_kv,new", [
+    (128, 6, 3, [130]), (128, 10, 5, [9, 1, 1]), (128, 64, 1, [1, 3]), (256, 12, 6, [40, 1]), (512, 7, 7, [33, 2])])
+@pytest.mark.parametrize("room", [0, 200_000, 3_000_000, 64 << 20])
+def test_attention_of_chunks_over_long_caches(ctx, f16, hd, n_q, n_kv, new, room):
+    """Row tiles cut into parts, with heads that do not divide the GPU and
+    workspaces for none, few and all of the parts."""
+    rng = np.random.default_rng(hd + n_kv)
+    page, kv = 64, [2000 + 700 * i for i in range(len(new))]
+    host, tables, cu = batch(rng, kv, new, page, n_kv, hd)
+    q = rng.standard_normal((cu[-1], n_q, hd)).astype(np.float16 if f16 else np.float32)
+    got = attend(ctx, to_pages(*host), torch.from_numpy(q).cuda(), tables, kv, cu, n_q, split=False,
+                 workspace=torch.empty(room, dtype=torch.uint8, device="cuda") if room else None)
+    want, mag, cond, peak = ref.attention(q, host[0], host[2], host[1], host[3], tables, kv, cu, 0, hd ** -0.5)
+    bound = ref.attention_bound(want, mag, cond, peak, hd, max(kv), f16)
+    assert (np.abs(got - want) <= bound).all()
+
+
+@gpu
+def test_a_captured_mixed_step_follows_its_lengths():
+    """One recording serves steps of different chunks: requests grow from nothing to
+    many rows and back to single tokens between the replays."""
+    import sgq
+    page, n_q, n_kv, hd, n, width, n_pages, rows = 32, 4, 2, 128, 4, 64, 200, 200
+    rng = np.random.default_rng(5)
+    side, gctx, ectx = torch.cuda.Stream(), sgq.GpuContext(0), sgq.GpuContext(0)
+
+    def fresh():
+        host = pool(np.random.default_rng(1), n_pages, n_kv, page, hd)
+        return dict(pages=to_pages(*host), lens=i32([0] * n), new=i32([0] * n), done=i32([0] * n),
+                    tables=i32(np.full((n, width), -1)), free=i32(np.arange(n_pages)), nf=i32([n_pages]),
+                    cu=i32([0] * (n + 1)), slots=i32([0] * rows), missing=i32([0]),
+                    k=torch.zeros((rows, n_kv, hd), device="cuda"), v=torch.zeros((rows, n_kv, hd), device="cuda"),
+                    q=torch.zeros((rows, n_q, hd), device="cuda"), out=torch.zeros((rows, n_q, hd), device="cuda"),
+                    ws=torch.empty(32 << 20, dtype=torch.uint8, device="cuda"))
+
+    def step(c, s):
+        c.kv_pages_release(s["done"], s["lens"], s["tables"], s["free"], s["nf"], page)
+        c.kv_pages_plan(s["lens"], s["new"], s["tables"], s["free"], s["nf"], s["nf"], s["lens"], s["cu"],
+                        s["slots"], s["missing"], page)
+        c.kv_append_paged_q8(s["pages"], s["k"], s["v"], s["slots"])
+        c.attn_paged_q8(s["pages"], s["q"], s["tables"], s["lens"], s["cu"], s["out"], max_new=rows,
+                        max_kv=width * page, workspace=s["ws"])
+
+    a, b = fresh(), fresh()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        gctx.set_stream(side)
+        with sgq.GraphRecorder(gctx) as rec:
+            step(gctx, a)
+    lens = np.zeros(n, int)
+    for i, (new, done) in enumerate([([150, 0, 1, 20], [0, 0, 0, 0]), ([1, 190, 1, 1], [0, 0, 0, 0]),
+                                     ([1, 1, 150, 40], [1, 0, 0, 0]), ([0, 0, 0, 0], [0, 0, 0, 1]),
+                                     ([1, 1, 1, 100], [0, 0, 0, 0])]):
+        x = [torch.from_numpy(rng.standard_normal(a[m].shape).astype(np.float32)) for m in "kvq"]
+        for s in (a, b):
+            for m, t in zip("kvq", x):
+                s[m].copy_(t)
+            s["new"].copy_(i32(new))
+            s["done"].copy_(i32(done))
+            s["out"].fill_(7.0)
+        torch.cuda.synchronize()
+        rec.graph.submit()
+        side.synchronize()
+        torch.ones(1 << 20, device="cuda").sum().item()  # eager work between the replays
+        step(ectx, b)
+        torch.cuda.synchronize()
+        lens = np.where(done, 0, lens) + new
+        for m in ("out", "lens", "tables", "slots", "nf", "cu"):
+            assert torch.equal(a[m], b[m]), (i, m)
+        assert a["lens"].tolist() == list(lens) and a["missing"].item() == 0
+        assert (a["out"][sum(new):] == 7.0).all() and not (a["out"][:sum(new)] == 7.0).all(-1).any()
+    del rec
+
+
+@gpu
 def test_two_streams_at_once(ctx):
     """Two contexts on two streams, each with its own cache and workspace."""
     import sgq
