@@ -8,10 +8,11 @@
 // position c_s + i, whose slot is table[s][pos/P]·P + pos%P.
 //
 // A few kilobytes: what counts is the launch and the chain of dependent
-// loads.  One workgroup scans both sums in LDS and pops the pages: the thread of
+// loads (64 requests 4.9 us, of which an empty kernel takes 2.4).  One workgroup scans both sums in LDS and pops the pages: the thread of
 // a page (or of a row) finds its request by bisection in the LDS sums.  It fills
 // the slot map too while that is one or two rows a thread (kPlanRows); a longer
-// one goes to a second launch over the whole GPU.
+// one goes to a second launch over the whole GPU (4 us for 32000 rows, 30 in one
+// workgroup).
 #include "paged.h"
 
 namespace sgq {
@@ -125,8 +126,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlan p) {
     }
     __syncthreads();
     // the popped pages
-    for (int i = tid; i < n_new; i += kPlanThreads) {
-        const int s = find_owner(pg_s, p.n_seqs, i);
+    for (uint32_t u = tid; u < (uint32_t)n_new; u += kPlanThreads) {  // n_new < 2^31
+        const int i = (int)u, s = find_owner(pg_s, p.n_seqs, i);
         const int have = (int)(((long long)cached_s[s] + P - 1) >> p.page_log2);
         const int at = n_free - 1 - i;
         p.tables[(size_t)s * p.max_pages + have + (i - pg_s[s])] = at >= 0 ? p.free_list[at] : -1;
@@ -158,44 +159,68 @@ __global__ __launch_bounds__(kRowsThreads) void paged_plan_rows_kernel(PagedPlan
     if (lost && (threadIdx.x & 63) == 0) atomicAdd(p.missing, lost);  // whole numbers: any order
 }
 
-// Pages go back in request order, a request's pages in table order.
+// Pages go back in request order, a request's pages in table order.  The finished
+// requests are listed first: what follows is bound by chains of LDS reads, and
+// a wave finds the owner of its 64 pages among them in two.  1024 requests, 128 of
+// them finished with 64 pages each: 15 us (a bisection per page, and counts
+// summed by every thread: 18).
 __global__ __launch_bounds__(kPlanThreads) void paged_release_kernel(PagedRelease p) {
-    __shared__ int pg_s[kPagedMaxSeqs + 1];
+    __shared__ int pg_s[kPagedMaxSeqs + 64];            // a finished request's first page
+    __shared__ unsigned short seq_s[kPagedMaxSeqs];
     __shared__ long long wave_s[kPlanThreads / 64];
-    const int P = 1 << p.page_log2, tid = threadIdx.x;
+    const int P = 1 << p.page_log2, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n_free = min(max(*p.n_free, 0), p.n_pages);
-    long long pg0 = 0;
+    constexpr int kCount = 40;  // a sum holds the pages below this bit, the requests from it on
+    long long sum0 = 0;
     for (int b = 0; b < p.n_seqs; b += kPlanThreads) {
         const int s = b + tid;
-        int held = 0;
-        if (s < p.n_seqs && p.done[s]) {
+        bool done = false;
+        long long held = 0;
+        if (s < p.n_seqs) {
             const long long h = ((long long)max(p.kv_lens[s], 0) + P - 1) >> p.page_log2;
-            held = (int)(h < p.max_pages ? h : p.max_pages);
+            done = p.done[s] != 0;
+            if (done) held = h < p.max_pages ? h : p.max_pages;
         }
         long long all;
-        const long long pg = pg0 + block_scan<kPlanThreads>(held, wave_s, &all);
-        if (s < p.n_seqs) pg_s[s] = clamp_len(pg - held);
-        pg0 += all;
+        const long long mine = held | (long long)done << kCount;
+        const long long before = sum0 + block_scan<kPlanThreads>(mine, wave_s, &all) - mine;
+        if (done) {
+            const int at = (int)(before >> kCount);
+            seq_s[at] = (unsigned short)s;
+            pg_s[at] = (int)(before & ((1ll << kCount) - 1));  // below 2^31, as the table's entries
+        }
+        sum0 += all;
     }
-    const int n_held = clamp_len(pg0);
-    if (tid == 0) pg_s[p.n_seqs] = n_held;
+    const int n_held = (int)(sum0 & ((1ll << kCount) - 1)), n_done = (int)(sum0 >> kCount);
+    if (tid < 64) pg_s[n_done + tid] = n_held;
     __syncthreads();
+    // The largest finished request that begins at or before page i0, by the whole wave.
+    const int stride = n_done / 64 + 1;
+    const auto owner_of = [&](int i0) {
+        const int hi = lane * stride;
+        const uint64_t a = __ballot(hi < n_done && pg_s[hi] <= i0);
+        const int from = max(__popcll(a) - 1, 0) * stride;
+        const uint64_t c = __ballot(lane < stride && from + lane < n_done && pg_s[min(from + lane, n_done)] <= i0);
+        return from + max(__popcll(c) - 1, 0);
+    };
     // entries outside the pool are dropped: the pushed ones are counted in order,
     // 8 rounds of a thread per page at a time
     constexpr int kRounds = 8, kWaves = kPlanThreads / 64;
+    static_assert(kRounds * kWaves == 128, "two a lane");
     __shared__ int count_s[kRounds * kWaves];
-    const int lane = tid & 63, wave = tid >> 6;
     int top = n_free;
-    for (int b = 0; b < n_held; b += kRounds * kPlanThreads) {
+    for (uint32_t b = 0; b < (uint32_t)n_held; b += kRounds * kPlanThreads) {  // n_held < 2^31
         int page[kRounds];
         uint64_t in[kRounds];
 #pragma unroll
         for (int k = 0; k < kRounds; k++) {
-            const int i = b + k * kPlanThreads + tid;
+            const int i = (int)(b + k * kPlanThreads + tid);
             page[k] = -1;
-            if (i >= 0 && i < n_held) {
-                const int s = find_owner(pg_s, p.n_seqs, i);
-                page[k] = p.tables[(size_t)s * p.max_pages + (i - pg_s[s])];
+            int o = owner_of(i - lane);
+            if ((uint32_t)i < (uint32_t)n_held) {
+                while (o + 1 < n_done && pg_s[o + 1] <= i) o++;
+                page[k] = p.tables[(size_t)seq_s[o] * p.max_pages + (i - pg_s[o])];
             }
         }
 #pragma unroll
@@ -208,32 +233,31 @@ __global__ __launch_bounds__(kPlanThreads) void paged_release_kernel(PagedReleas
             count_s[lane * kWaves + wave] = __popcll(mine);
         }
         __syncthreads();
-        int at = top;
+        // sums over the 128 counts, two a lane
+        const int c0 = count_s[lane], c1 = count_s[64 + lane];
+        int s0 = c0, s1 = c1;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o0 = __shfl_up(s0, d), o1 = __shfl_up(s1, d);
+            s0 += lane >= d ? o0 : 0;
+            s1 += lane >= d ? o1 : 0;
+        }
+        const int half = __builtin_amdgcn_readlane(s0, 63);
 #pragma unroll
         for (int k = 0; k < kRounds; k++) {
-            int before = 0, all = 0;
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) {
-                const int c = count_s[k * kWaves + w];
-                before += w < wave ? c : 0;
-                all += c;
-            }
-            const int to = at + before + __popcll(in[k] & ((1ull << lane) - 1));
+            const int before = k < kRounds / 2 ? __builtin_amdgcn_readlane(s0 - c0, k * kWaves + wave)
+                                               : half + __builtin_amdgcn_readlane(s1 - c1, k * kWaves - 64 + wave);
+            const int to = top + before + __popcll(in[k] & ((1ull << lane) - 1));
             if (in[k] >> lane & 1 && to < p.n_pages) p.free_list[to] = page[k];
-            at += all;
         }
-        top = min(at, p.n_pages);
+        top = min(top + half + __builtin_amdgcn_readlane(s1, 63), p.n_pages);
     }
-    __syncthreads();
-    // a wave clears the rows of 64 requests: only finished ones cost a store
-    for (int b = (tid >> 6) * 64; b < p.n_seqs; b += kPlanThreads) {
-        const int s = b + (tid & 63);
-        const bool done = s < p.n_seqs && p.done[s];
-        if (done) p.kv_lens[s] = 0;
-        for (uint64_t m = __ballot(done); m; m &= m - 1) {
-            int32_t *row = p.tables + (size_t)(b + __builtin_ctzll(m)) * p.max_pages;
-            for (int j = tid & 63; j < p.max_pages; j += 64) row[j] = -1;
-        }
+    __syncthreads();  // the tables have been read
+    for (int d = wave; d < n_done; d += kWaves) {
+        const int s = seq_s[d];
+        if (lane == 0) p.kv_lens[s] = 0;
+        int32_t *row = p.tables + (size_t)s * p.max_pages;
+        for (int j = lane; j < p.max_pages; j += 64) row[j] = -1;
     }
     if (tid == 0) *p.n_free = top;
 }
