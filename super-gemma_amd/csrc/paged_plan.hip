@@ -8,18 +8,19 @@
 // position c_s + i, whose slot is table[s][pos/P]·P + pos%P.
 //
 // A few kilobytes: what counts is the launch and the chain of dependent
-// loads (64 requests 4.9 us, of which an empty kernel takes 2.4).  One workgroup scans both sums in LDS and pops the pages: the thread of
-// a page (or of a row) finds its request by bisection in the LDS sums.  It fills
-// the slot map too while that is one or two rows a thread (kPlanRows); a longer
-// one goes to a second launch over the whole GPU (4 us for 32000 rows, 30 in one
-// workgroup).
+// loads (64 requests: 4.9 us, of which an empty kernel takes 2.4).  One workgroup
+// scans both sums in LDS and pops the pages: the thread of a page (or of a row)
+// finds its request by bisection in the LDS sums.  It fills the slot map too up to
+// four rows a thread; a longer one goes to a second launch over the whole GPU
+// (64 rows: 8.4 us in one launch, 13.7 in two; 4060 rows: 27.7 and 30.5, with a
+// release; 8100: 29.2 and 29.3; 32000: 64 and 35).
 #include "paged.h"
 
 namespace sgq {
 namespace {
 
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanRows = 2 * kPlanThreads;
+constexpr int kPlanRows = 4 * kPlanThreads;
 
 // Inclusive sums over the workgroup of one value a thread.
 template <int NT>
