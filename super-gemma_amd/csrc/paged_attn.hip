@@ -27,7 +27,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNoMax = -1e30f;      // the reference M before the first key
 // M moves only when a tile's maximum is over it by this (log2); weights are
 // taken against M - kHead, so f16 weights lie below 2^(kLazy + kHead) = 2^14
-// and their subnormals begin 2^20 below M.
+// and their subnormals begin 2^20 below M.  (Two prompts of 4001 rows: 335 us;
+// with M moved at every larger score 389.)
 constexpr float kLazy = 8.f, kHead = 6.f;
 constexpr float kMinScale = 0x1p-100f;  // V scales below weigh as this one
 
@@ -60,7 +61,9 @@ struct RowTile {
 __device__ __forceinline__ int clamped(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
 // Requests with at most kFewRows rows a kv head (single tokens) share a wave's
-// 16 columns; their keys are what is spread over the GPU.
+// 16 columns; their keys are what is spread over the GPU, and their quants go from
+// memory to registers.  Through the kernel of many rows, whose waves share keys
+// in LDS, 64 single tokens over up to 8192 keys take 624 us in place of 244.
 constexpr int kFewRows = 16;
 
 __device__ __forceinline__ bool request_rows(const AttnArgs &a, int seq, RowTile *t) {
@@ -235,7 +238,8 @@ __device__ __forceinline__ h8 quants_f16(uint32_t w0, uint32_t w1) {
 }
 
 // 8 quants as the f16 numbers (q + 128)·2^-24: the byte is a subnormal's bits.
-// Exact, at 6 operations in place of 10; who takes these subtracts the 128.
+// Exact, at 6 operations in place of 10; who takes these subtracts the 128 (12 single
+// tokens over up to 32768 keys of 512 dims: 208 us, with the 10 operations 249).
 __device__ __forceinline__ h8 quants_f16_raised(uint32_t w0, uint32_t w1) {
     const uint32_t x0 = w0 ^ 0x80808080u, x1 = w1 ^ 0x80808080u;
     const uint4 p = make_uint4(__builtin_amdgcn_perm(0, x0, 0x0c010c00u), __builtin_amdgcn_perm(0, x0, 0x0c030c02u),
@@ -454,7 +458,9 @@ struct Wave {
     }
 
     // Tiles t0, t0 + step, ... below t1.  STREAM: no other wave reads these pages
-    // soon, so they are not kept in the caches.
+    // soon, so they are not kept in the caches (64 requests of up to 8192 keys, 16 heads
+    // of 128: 243 us, kept 256; one of 32768: 29 and 33).  Not at 512 dims, where that
+    // is the slower way (12 requests of up to 32768, 4 heads: 197 us, kept 184).
     template <bool STREAM>
     __device__ __forceinline__ void attend(const AttnArgs &a, const RowTile &rt, int head, int t0, int t1,
                                            int step, int lane) {
@@ -557,7 +563,11 @@ __device__ __forceinline__ size_t few_row(const AttnArgs &a, const RowTile &rt, 
 }
 
 // Few rows: one request and kv head against one part of the keys, the tiles dealt
-// to 4 waves in turn and their sums joined in LDS in wave order.
+// to 4 waves in turn and their sums joined in LDS in wave order.  Bound by reading
+// the pages: 64 single tokens over up to 8192 keys (16 heads of 128, f16) 244 us,
+// 5.5 TB/s; 12 over up to 32768 (4 heads of 512) 184 us, 5.6 TB/s; one over 8191
+// (fp32) 13 us with the join, of which the launches and the latency of the first loads
+// are 8.
 constexpr int kFewWaves = 4;
 
 template <typename T, int HD>
@@ -587,7 +597,7 @@ __global__ __launch_bounds__(kFewWaves * 64, HD == 128 ? 3 : HD == 256 ? 2 : 1) 
         __syncthreads();
         w.ql_s = ql_s;
     }
-    w.template attend<true>(a, rt, head, t0 + wave, t1, kFewWaves, lane);
+    w.template attend<HD != 512>(a, rt, head, t0 + wave, t1, kFewWaves, lane);
     if (g == 0) {
         ml_s[wave][0][n] = w.M[0];
         ml_s[wave][1][n] = w.l[0];
@@ -641,7 +651,12 @@ __global__ __launch_bounds__(kFewWaves * 64, HD == 128 ? 3 : HD == 256 ? 2 : 1) 
 //   K [key][HD]: the 16-byte units of a row are stored at unit ^ swizzle(key), so
 //                that the 16 keys of a fragment read fall on different banks
 //   V [tile][dim][32 keys]: a fragment is one kilobyte, its four units of a dim
-//                likewise exchanged
+//                likewise exchanged (2048 rows of 256 dims: 113 us, else 120)
+// The products of f16 rows of 128 dims have 32 rows a wave, at half the LDS reads
+// of 16 (two prompts of 4001 rows: 335 us and 440), four reads ahead (two: 356); wider
+// rows' accumulators leave no room for that.  Bound by LDS reads and the
+// scores' vector work beside the products: the prompts run at 780 - 840 TFLOP/s, 1111 fp32
+// rows of 256 dims with a window, at two products each, at 310 (620 done).
 template <typename T, int HD>
 struct Many {
     static constexpr bool F32 = sizeof(T) == 4;
@@ -971,8 +986,9 @@ __global__ __launch_bounds__(kJoinWaves * 64) void paged_attn_join_kernel(AttnAr
 // How a call is laid out: which kernels run, and into how many parts at most
 // they cut the keys of a row.
 int few_cap(int max_new, int group) { return (int)std::min<long long>((long long)max_new * group, kFewRows); }
-// Parts of many rows, together: three rounds.
-constexpr int kManyParts = 3 * kCus;
+// Parts of many rows, together: two rounds (768 rows over 16384 keys, 96 workgroups
+// uncut: 305 us with parts for one round, 282 for two, 283 for three).
+constexpr int kManyParts = 2 * kCus;
 constexpr int kJoinWgs = 8 * kCus;  // of many rows: as many as fit
 struct Layout {
     bool few, many;
