@@ -313,7 +313,7 @@ __global__ __launch_bounds__(kAppThreads) void paged_gather_kernel(
 template <typename T, int HD>
 int append(hipStream_t st, const PagedPages &pg, const void *k, uint64_t k_stride, const void *v,
            uint64_t v_stride, const int32_t *slots, int n) {
-    // Single tokens want a workgroup each (16 heads of 128, 128 requests: 16 us with windows
+    // Single tokens want a workgroup each (16 heads of 128, 64 requests: 16 us with windows
     // of 1, 24 of 8, 59 of 32), runs as few empty workgroups as possible (a prompt of
     // 2040 rows: 56 us of 1, 34 of 8, 27 of 32; 4096 rows: 42 of 63, 53 of 32).  Many
     // rows are more often prompts: 64 windows, until a wave's 64 slots hold no more.
