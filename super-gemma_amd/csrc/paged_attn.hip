@@ -897,11 +897,11 @@ __global__ __launch_bounds__((Many<T, HD>::kThreads), (Many<T, HD>::kWaves / 4))
 // and are summed in wave order.  The lanes share out the parts' references and
 // sums, then the dims.
 constexpr int kJoinWaves = 4;
-template <typename T, int HD, int W>
+template <typename T, int HD>
 __device__ __forceinline__ void join_row(const AttnArgs &a, const RowTile &rt, int head, int i, int parts,
                                          const float *part, const float2 *part_ml, size_t prow) {
-    constexpr int ND = HD / 64;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W;
+    constexpr int ND = HD / 64, W = kJoinWaves;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = rt.row0 + i, tok = rt.tok0 + r / a.group, qh = head * a.group + r % a.group;
     float m = kNoMax, l = 0.f, o[ND];
     for (int s = lane; s < parts; s += 64) m = fmaxf(m, part_ml[prow + s].x);
@@ -931,22 +931,58 @@ __device__ __forceinline__ void join_row(const AttnArgs &a, const RowTile &rt, i
         }
     }
     T *dst = static_cast<T *>(a.out) + (size_t)tok * a.out_stride + (size_t)qh * HD;
-    if constexpr (W == 1) {
+    static_assert(W == 4, "the sums below");
+    __shared__ float o_s[W][HD], l_s[W];
+#pragma unroll
+    for (int d = 0; d < ND; d++) o_s[wave][d * 64 + lane] = o[d];
+    if (lane == 0) l_s[wave] = l;
+    __syncthreads();
+    const float inv = inverse(l_s[0] + l_s[1] + l_s[2] + l_s[3]);
+    for (int d = threadIdx.x; d < HD; d += W * 64)
+        dst[d] = (T)((o_s[0][d] + o_s[1][d] + o_s[2][d] + o_s[3][d]) * inv);
+}
+
+// Row i0 + lane/L of a cut tile, L lanes a row (two rows a wave at 128 dims, in flight
+// together): all parts, four at a time.
+template <typename T, int HD>
+struct ManyJoin {
+    static constexpr int L = HD / 4 < 64 ? HD / 4 : 64, kRows = 64 / L, NV = HD / 4 / L;
+    static __device__ __forceinline__ void rows(const AttnArgs &a, const RowTile &rt, int head, int i0, int parts,
+                                                const float *part, const float2 *part_ml, size_t prow0, int splits) {
+        const int lane = threadIdx.x & 63, c = lane % L, i = i0 + lane / L;
+        const bool live = i < rt.rows;
+        const size_t prow = prow0 + (size_t)(live ? lane / L : 0) * splits;
+        float m = kNoMax, l = 0.f;
+        for (int s = 0; s < parts; s += 4)
+#pragma unroll
+            for (int k = 0; k < 4; k++) m = fmaxf(m, part_ml[prow + min(s + k, parts - 1)].x);
+        f4 o[NV] = {};
+        for (int s = 0; s < parts; s += 4) {
+            f4 v[4][NV];
+            float2 ml[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const size_t p = prow + min(s + k, parts - 1);
+                ml[k] = part_ml[p];
+#pragma unroll
+                for (int d = 0; d < NV; d++) v[k][d] = *reinterpret_cast<const f4 *>(part + p * HD + (d * L + c) * 4);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float f = s + k < parts ? __builtin_amdgcn_exp2f(ml[k].x - m) : 0.f;
+                l = s + k < parts ? fmaf(ml[k].y, f, l) : l;
+#pragma unroll
+                for (int d = 0; d < NV; d++) o[d] = s + k < parts ? o[d] + v[k][d] * f : o[d];
+            }
+        }
+        if (!live) return;
+        const int r = rt.row0 + i, tok = rt.tok0 + r / a.group, qh = head * a.group + r % a.group;
+        T *dst = static_cast<T *>(a.out) + (size_t)tok * a.out_stride + (size_t)qh * HD;
         const float inv = inverse(l);
 #pragma unroll
-        for (int d = 0; d < ND; d++) dst[d * 64 + lane] = (T)(o[d] * inv);
-    } else {
-        static_assert(W == 4, "the sums below");
-        __shared__ float o_s[W][HD], l_s[W];
-#pragma unroll
-        for (int d = 0; d < ND; d++) o_s[wave][d * 64 + lane] = o[d];
-        if (lane == 0) l_s[wave] = l;
-        __syncthreads();
-        const float inv = inverse(l_s[0] + l_s[1] + l_s[2] + l_s[3]);
-        for (int d = threadIdx.x; d < HD; d += W * 64)
-            dst[d] = (T)((o_s[0][d] + o_s[1][d] + o_s[2][d] + o_s[3][d]) * inv);
+        for (int d = 0; d < NV; d++) store4(dst + (d * L + c) * 4, scaled(o[d], inv));
     }
-}
+};
 
 // Many rows have few parts: the waves of n_many workgroups take them in turn.  Few
 // rows have many: a workgroup a row of a single token.
@@ -961,8 +997,8 @@ __global__ __launch_bounds__(kJoinWaves * 64) void paged_attn_join_kernel(AttnAr
         const KeySpan ks = key_span(a, rt, a.few_splits, a.few_per);
         if (ks.parts == 1 || i >= rt.rows) return;
         for (;;) {
-            join_row<T, HD, kJoinWaves>(a, rt, head, i, ks.parts, a.few_part, a.few_ml,
-                                        few_row(a, rt, head, i) * a.few_splits);
+            join_row<T, HD>(a, rt, head, i, ks.parts, a.few_part, a.few_ml,
+                            few_row(a, rt, head, i) * a.few_splits);
             i += each;
             if (i >= rt.rows) break;
             __syncthreads();  // its LDS is read
@@ -973,13 +1009,14 @@ __global__ __launch_bounds__(kJoinWaves * 64) void paged_attn_join_kernel(AttnAr
     ManyScan<BM> scan;
     const ManyPlan plan = many_plan<BM, HD>(a, scan);
     const int units = (plan.tiles - plan.whole) * a.pg.n_kv;
-    const int first = blockIdx.x * kJoinWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int w = first; w < units * BM; w += n_many * kJoinWaves) {
+    using J = ManyJoin<T, HD>;
+    const int first = (blockIdx.x * kJoinWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * J::kRows;
+    for (int w = first; w < units * BM; w += n_many * kJoinWaves * J::kRows) {
         const int unit = w / BM, i = w % BM, head = unit % a.pg.n_kv;
         if (!many_rows(a, scan, plan.tiles - 1 - plan.whole - unit / a.pg.n_kv, &rt) || i >= rt.rows) continue;
         const KeySpan ks = key_span(a, rt, plan.splits, plan.per);
         if (ks.parts > 1)
-            join_row<T, HD, 1>(a, rt, head, i, ks.parts, a.many_part, a.many_ml, (size_t)w * plan.splits);
+            J::rows(a, rt, head, i, ks.parts, a.many_part, a.many_ml, (size_t)w * plan.splits, plan.splits);
     }
 }
 
@@ -1061,7 +1098,7 @@ int launch(hipStream_t st, const AttnArgs &a, const Layout &y) {
     const int each = std::min(a.group, a.few_cap), n_few = a.few_splits > 1 ? a.n_seqs * a.pg.n_kv * each : 0;
     if (a.many_room > 1) {
         const long long units = std::min<long long>(a.many_room / 2, (long long)a.many_tiles * a.pg.n_kv);
-        const int n_many = (int)std::min<long long>(kJoinWgs, units * Many<T, HD>::kRows / kJoinWaves);
+        const int n_many = (int)std::min<long long>(kJoinWgs, units * Many<T, HD>::kRows / (kJoinWaves * ManyJoin<T, HD>::kRows));
         hipLaunchKernelGGL((paged_attn_join_kernel<T, HD, true>), dim3(n_many + n_few), dim3(kJoinWaves * 64), 0, st, a,
                            n_many);
         SGQ_HIP(hipGetLastError());
