@@ -572,9 +572,11 @@ constexpr int kFewWaves = 4;
 
 template <typename T, int HD>
 __global__ __launch_bounds__(kFewWaves * 64, HD == 128 ? 3 : HD == 256 ? 2 : 1) void paged_attn_few_kernel(AttnArgs a) {
-    constexpr int NC = HD / 64;
+    // dims that the waves' sums meet in LDS at a time: few barriers, and room for the
+    // workgroups that a CU's registers hold
+    constexpr int CW = HD == 512 ? 256 : 128;
     __shared__ float ml_s[kFewWaves][2][16];
-    __shared__ __align__(16) float o_s[kFewWaves][16][64 + 4];
+    __shared__ __align__(16) float o_s[kFewWaves][16][CW + 4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     // the heads of a page lie side by side, and so do their workgroups
     const int head = blockIdx.x % a.pg.n_kv, unit = blockIdx.x / a.pg.n_kv;
@@ -590,6 +592,7 @@ __global__ __launch_bounds__(kFewWaves * 64, HD == 128 ? 3 : HD == 256 ? 2 : 1) 
         // both halves of q, the accumulator and a tile on its way are more registers than
         // a wave has (84 spilled): the waves' common low half from LDS, 174 -> 119 us
         // for 16 requests of 8192 keys
+        constexpr int NC = HD / 64;
         __shared__ h8 ql_s[NC * 2][64];
         if (wave == 0)
 #pragma unroll
@@ -618,21 +621,24 @@ __global__ __launch_bounds__(kFewWaves * 64, HD == 128 ? 3 : HD == 256 ? 2 : 1) 
     const size_t prow = few_row(a, rt, head, orow) * a.few_splits + split;
     const float inv = inverse(ol);
 #pragma unroll
-    for (int c = 0; c < NC; c++) {
+    for (int c = 0; c < HD / CW; c++) {
+        if (c) __syncthreads();
+#pragma unroll
+        for (int d = 0; d < CW / 16; d++)
+            store4(&o_s[wave][n][d * 16 + g * 4], scaled(w.acc[0][c * (CW / 16) + d], f));
         __syncthreads();
 #pragma unroll
-        for (int d = 0; d < 4; d++) store4(&o_s[wave][n][d * 16 + g * 4], scaled(w.acc[0][c * 4 + d], f));
-        __syncthreads();
-        f4 o = f4{0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < CW; k += 64) {
+            if (orow >= rt.rows) break;
+            f4 o = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < kFewWaves; i++) o += *reinterpret_cast<const f4 *>(&o_s[i][orow][od]);
-        if (orow < rt.rows) {
+            for (int i = 0; i < kFewWaves; i++) o += *reinterpret_cast<const f4 *>(&o_s[i][orow][k + od]);
+            const int dim = c * CW + k + od;
             if (ks.parts == 1) {
-                store4(static_cast<T *>(a.out) + (size_t)otok * a.out_stride + (size_t)oh * HD + c * 64 + od,
-                       scaled(o, inv));
+                store4(static_cast<T *>(a.out) + (size_t)otok * a.out_stride + (size_t)oh * HD + dim, scaled(o, inv));
             } else {
-                store4(a.few_part + prow * HD + c * 64 + od, scaled(o, 1.f));
-                if (c == 0 && od == 0) a.few_ml[prow] = make_float2(om, ol);
+                store4(a.few_part + prow * HD + dim, scaled(o, 1.f));
+                if (dim == 0) a.few_ml[prow] = make_float2(om, ol);
             }
         }
     }
@@ -1047,6 +1053,17 @@ int splits_for(int units, int head_dim, int max_kv) {
     return std::clamp(by_fill, 1, std::max(by_keys, 1));
 }
 
+// Into how many parts `units` workgroups over `keys` 32-key tiles are best cut.
+int best_parts(int units, int keys, int area) {
+    int best = 1;
+    float least = parts_cost(units, 1, keys, area);
+    for (int p = 2; p <= 64 && keys / p >= 4 && units * p <= kManyParts; p++) {
+        const float us = parts_cost(units, p, (keys + p - 1) / p, area);
+        if (us < least) least = us, best = p;
+    }
+    return units ? best : 1;
+}
+
 Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f16, int max_new, int max_kv) {
     const int group = n_q / n_kv;
     Layout y{};
@@ -1067,18 +1084,12 @@ Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f1
         // a request with many rows has more than kFewRows, and a last tile that is not full
         const int last = y.few ? (int)std::min<long long>(n_seqs, (long long)n_tokens * group / (kFewRows + 1)) : 1;
         y.many_tiles = (int)((long long)n_tokens * group / y.many_bm) + std::max(last, 1);
-        y.many_parts = std::min<long long>(kManyParts, 64ll * y.many_tiles * n_kv);
-        if (n_seqs == 1) {  // its rows are known, and so are its parts
-            const int tiles = (int)(((long long)n_tokens * group + y.many_bm - 1) / y.many_bm);
-            const int units = (tiles - whole_tiles(tiles, n_kv)) * n_kv, keys = max_kv / 32 + 1;
-            float least = parts_cost(units, 1, keys, y.many_bm * head_dim);
-            int best = 0;
-            for (int p = 2; p <= 64 && keys / p >= 4 && units * p <= y.many_parts; p++) {
-                const float us = parts_cost(units, p, (keys + p - 1) / p, y.many_bm * head_dim);
-                if (us < least) least = us, best = p;
-            }
-            y.many_parts = units * best;
-        }
+        // The remainder of a lone request is known, and so are its parts.  Of several it
+        // is n_kv at least: no room (and no join) where even that is not worth a cut.
+        const int tiles = (int)(((long long)n_tokens * group + y.many_bm - 1) / y.many_bm);
+        const int units = n_seqs == 1 ? (tiles - whole_tiles(tiles, n_kv)) * n_kv : n_kv;
+        const int cut = best_parts(units, max_kv / 32 + 1, y.many_bm * head_dim);
+        if (cut > 1) y.many_parts = n_seqs == 1 ? units * cut : (int)std::min<long long>(kManyParts, 64ll * y.many_tiles * n_kv);
     }
     return y;
 }
