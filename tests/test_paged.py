@@ -196,6 +196,32 @@ def test_append_of_long_runs(ctx, n):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("n", [130, 900, 2100, 4300])
+def test_append_of_mixed_runs(ctx, n, dtype):
+    """Runs of all lengths, in and out of order, with slots named twice and rows
+    without one between them: many runs begin in a workgroup's window."""
+    rng = np.random.default_rng(n)
+    page, hd, n_kv = 64, 128, 2
+    slots, p = [], 0
+    while len(slots) < n:
+        m = int(rng.choice([1, 1, 1, 2, 17, 40, 64]))
+        a = int(rng.integers(0, page - m + 1))
+        run = [p * page + a + i for i in range(m)]
+        kind = rng.integers(0, 4)
+        if kind == 1:
+            run = run[::-1]
+        elif kind == 2:
+            run = [run[i] for i in rng.integers(0, m, m)]
+        slots += run + ([-1] * int(rng.integers(1, 4)) if rng.random() < 0.2 else [])
+        p += 1
+    host = pool(rng, p + 1, n_kv, page, hd)
+    x = [(rng.standard_normal((len(slots), n_kv, hd)) * s).astype(dtype) for s in (1.0, 3.0)]
+    pages, want = run_append(ctx, host, x, slots)
+    assert_pages(pages, want)
+
+
+@gpu
 def test_append_special_values(ctx):
     """All-zero rows, subnormal and huge ones, ties, infinities and NaN; a block
     with a NaN scale stays so until it begins anew; a slot named twice takes the
@@ -611,6 +637,46 @@ def test_a_captured_decode_step_replays_with_growing_lengths():
             assert torch.equal(a[m], b[m]), (i, m)
         assert a["lens"].tolist() == [s + i + 1 for s in start] and a["missing"].item() == 0
     del rec
+
+
+@gpu
+@pytest.mark.parametrize("f16", [True, False])
+def test_a_very_long_prompt(ctx, f16):
+    """70001 tokens of one request planned, appended and attended in one step; rows from
+    its start to its end are checked."""
+    page, n_q, n_kv, hd, n, width = 128, 2, 1, 128, 70001, 600
+    import sgq
+    rng = np.random.default_rng(77)
+    dt = np.float16 if f16 else np.float32
+    q, k, v = (rng.standard_normal((n, h, hd)).astype(dt) for h in (n_q, n_kv, n_kv))
+    pages = sgq.KvPages.empty(width, page, n_kv, hd)
+    lens, tables, cu, slots, missing = i32([0]), i32(np.full((1, width), -1)), i32([0, 0]), i32([0] * n), i32([9])
+    nf = i32([width])
+    ctx.kv_pages_plan(lens, i32([n]), tables, i32(rng.permutation(width)), nf, nf, lens, cu, slots, missing, page)
+    qd, kd, vd = (torch.from_numpy(x).cuda() for x in (q, k, v))
+    ctx.kv_append_paged_q8(pages, kd, vd, slots)
+    got = attend(ctx, pages, qd, tables.cpu().numpy(), [n], np.array([0, n]), n_q)
+    assert missing.item() == 0 and lens.item() == n and nf.item() == width - -(-n // page)
+    table = tables.cpu().numpy()
+    kq, vq, ks, vs = from_pages(pages)
+    for x, quants, d in ((k, kq, ks), (v, vq, vs)):  # runs of whole pages: half a step of the block's scale
+        for row in rng.integers(0, n, 300):
+            p, o = table[0, row // page], row % page
+            run = x[row // page * page:row // page * page + page].astype(np.float64)
+            assert d[p, 0] == np.float32(np.abs(run).max().astype(np.float32) / np.float32(127))
+            assert (quants[p, 0, o] == np.rint(x[row, 0].astype(np.float64) / np.float64(d[p, 0]))).all()
+    for row in (0, 1, 127, 128, 4095, 35000, 69888, n - 1):
+        want, mag, cond, peak = ref.attention(q[row:row + 1], kq, ks, vq, vs, table, [row + 1], np.array([0, 1]), 0,
+                                              hd ** -0.5)
+        bound = ref.attention_bound(want, mag, cond, peak, hd, row + 1, f16)
+        assert (np.abs(got[row:row + 1] - want) <= bound).all(), row
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 20])
+def test_attention_of_many_heads(ctx, new):
+    """1024 kv heads: more units than a round of the GPU has workgroups."""
+    check_attention(ctx, 3, [41], [new], 32, 1024, 1024, 128, True)
 
 
 @gpu
