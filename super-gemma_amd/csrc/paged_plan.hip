@@ -161,12 +161,12 @@ __global__ __launch_bounds__(kRowsThreads) void paged_plan_rows_kernel(PagedPlan
 }
 
 // Pages go back in request order, a request's pages in table order.  The finished
-// requests are listed first: what follows is bound by chains of LDS reads, and
-// a wave finds the owner of its 64 pages among them in two.  1024 requests, 128 of
-// them finished with 64 pages each: 15 us (a bisection per page, and counts
-// summed by every thread: 18).
+// requests are listed first, and a wave writes where its requests' entries are:
+// what follows is bound by chains of LDS reads and loads.  1024 requests, 128 of them
+// finished with 64 pages each: 11.6 us (a bisection per page, and counts summed by
+// every thread: 18).
 __global__ __launch_bounds__(kPlanThreads) void paged_release_kernel(PagedRelease p) {
-    __shared__ int pg_s[kPagedMaxSeqs + 64];            // a finished request's first page
+    __shared__ int pg_s[kPagedMaxSeqs + 1];             // a finished request's first page
     __shared__ unsigned short seq_s[kPagedMaxSeqs];
     __shared__ long long wave_s[kPlanThreads / 64];
     const int P = 1 << p.page_log2, tid = threadIdx.x, lane = tid & 63;
@@ -194,35 +194,29 @@ __global__ __launch_bounds__(kPlanThreads) void paged_release_kernel(PagedReleas
         sum0 += all;
     }
     const int n_held = (int)(sum0 & ((1ll << kCount) - 1)), n_done = (int)(sum0 >> kCount);
-    if (tid < 64) pg_s[n_done + tid] = n_held;
+    if (tid == 0) pg_s[n_done] = n_held;
     __syncthreads();
-    // The largest finished request that begins at or before page i0, by the whole wave.
-    const int stride = n_done / 64 + 1;
-    const auto owner_of = [&](int i0) {
-        const int hi = lane * stride;
-        const uint64_t a = __ballot(hi < n_done && pg_s[hi] <= i0);
-        const int from = max(__popcll(a) - 1, 0) * stride;
-        const uint64_t c = __ballot(lane < stride && from + lane < n_done && pg_s[min(from + lane, n_done)] <= i0);
-        return from + max(__popcll(c) - 1, 0);
-    };
     // entries outside the pool are dropped: the pushed ones are counted in order,
     // 8 rounds of a thread per page at a time
     constexpr int kRounds = 8, kWaves = kPlanThreads / 64;
     static_assert(kRounds * kWaves == 128, "two a lane");
     __shared__ int count_s[kRounds * kWaves];
+    __shared__ int entry_s[kRounds * kPlanThreads];  // of these rounds' pages, in the tables
     int top = n_free;
     for (uint32_t b = 0; b < (uint32_t)n_held; b += kRounds * kPlanThreads) {  // n_held < 2^31
         int page[kRounds];
         uint64_t in[kRounds];
+        const uint32_t end = min(b + kRounds * kPlanThreads, (uint32_t)n_held);
+        for (int d = wave; d < n_done; d += kWaves) {
+            const uint32_t lo = max((uint32_t)pg_s[d], b), hi = min((uint32_t)pg_s[d + 1], end);
+            const uint32_t first = (uint32_t)(seq_s[d] * p.max_pages) - (uint32_t)pg_s[d];  // wraps, and back
+            for (uint32_t i = lo + lane; i < hi; i += 64) entry_s[i - b] = (int)(first + i);
+        }
+        __syncthreads();
 #pragma unroll
         for (int k = 0; k < kRounds; k++) {
-            const int i = (int)(b + k * kPlanThreads + tid);
-            page[k] = -1;
-            int o = owner_of(i - lane);
-            if ((uint32_t)i < (uint32_t)n_held) {
-                while (o + 1 < n_done && pg_s[o + 1] <= i) o++;
-                page[k] = p.tables[(size_t)seq_s[o] * p.max_pages + (i - pg_s[o])];
-            }
+            const int at = k * kPlanThreads + tid;
+            page[k] = b + at < end ? p.tables[entry_s[at]] : -1;
         }
 #pragma unroll
         for (int k = 0; k < kRounds; k++) in[k] = __ballot((unsigned)page[k] < (unsigned)p.n_pages);

@@ -130,6 +130,29 @@ def test_release_leaves_out_missing_pages_and_keeps_the_stack_in_bounds(ctx):
     assert t[4].item() == 7 and np.array_equal(t[3].cpu().numpy(), free)
 
 
+@gpu
+@pytest.mark.parametrize("n,width", [(400, 90), (3, 20011), (4096, 30)])
+def test_release_of_many_pages(ctx, n, width):
+    """More pages than one round of the workgroup takes, some of them missing or
+    outside the pool, by requests with none, few and more than their table holds."""
+    rng = np.random.default_rng(n)
+    page, n_pages = 64, n * width
+    kv = rng.integers(0, page * (width + 5), n)
+    kv[rng.random(n) < 0.2] = 0
+    kv[0] = page * width
+    tables = rng.permutation(n_pages).reshape(n, width).astype(np.int32)
+    tables[rng.random((n, width)) < 0.03] = -1
+    tables[rng.random((n, width)) < 0.01] = n_pages
+    done = (rng.random(n) < 0.8).astype(np.int32)
+    done[0] = 1
+    free, n_free = np.full(n_pages, -7, np.int32), 5
+    t = [i32(done), i32(kv), i32(tables), i32(free), i32([n_free])]
+    ctx.kv_pages_release(*t, page)
+    want = ref.release(done, kv, tables, free, n_free, page)
+    for got, w in zip(t[1:], want):
+        assert np.array_equal(got.cpu().numpy().reshape(-1), np.asarray(w, np.int32).reshape(-1))
+
+
 # ---- append and read-back -----------------------------------------------------------
 
 def run_append(ctx, host, x, slots, fused=False, skip=True):
