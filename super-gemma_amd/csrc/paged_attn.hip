@@ -24,7 +24,7 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kNoMax = -1e30f;      // the reference M before the first key
+constexpr float kNoMax = -3.4e38f;    // the reference M before the first key: below any score
 // M moves only when a tile's maximum is over it by this (log2); weights are
 // taken against M - kHead, so f16 weights lie below 2^(kLazy + kHead) = 2^14
 // and their subnormals begin 2^20 below M.  (Two prompts of 4001 rows: 335 us;
@@ -377,41 +377,37 @@ struct Wave {
                                           const float (&sc)[K][3], const f4 (&s)[K][NT][2], h8 (&w)[K][NT],
                                           h8 (&wl)[K][F32 ? NT : 1], int n, int g) {
         float x[K][NT][8], mx = -INFINITY;
-        const auto score = [&]() {
-            mx = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < K; k++)
+        for (int k = 0; k < K; k++)
 #pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    const float c = row_scale[j] * sc[k][0];
-                    const float b = fmaf(row_raise[j], sc[k][0], sc[k][1] + (kHead - M[j]));
+            for (int j = 0; j < NT; j++) {
+                const float c = row_scale[j] * sc[k][0];
+                const float b = fmaf(row_raise[j], sc[k][0], sc[k][1] + (kHead - M[j]));
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[k][j][e] = fmaf(s[k][j][e >> 2][e & 3], c, b);
-                }
-            if (edge) {
-                asm volatile("");  // a branch: as selects the masks would be half of the loop's VALU work
-#pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    const int row = rt.row0 + min(j * 16 + n, rt.rows - 1);
-                    const int pos = rt.pos0 + row / a.group;
-                    const int lo = key_lo(a, pos), hi = min(key_hi(a, pos, rt.kv_len), key_end);
-#pragma unroll
-                    for (int k = 0; k < K; k++)
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const int key = (t + k) * 32 + g * 8 + e;
-                            x[k][j][e] = key >= lo && key < hi ? x[k][j][e] : -INFINITY;
-                        }
-                }
+                for (int e = 0; e < 8; e++) x[k][j][e] = fmaf(s[k][j][e >> 2][e & 3], c, b);
             }
+        if (edge) {
+            asm volatile("");  // a branch: as selects the masks would be half of the loop's VALU work
 #pragma unroll
-            for (int k = 0; k < K; k++)
+            for (int j = 0; j < NT; j++) {
+                const int row = rt.row0 + min(j * 16 + n, rt.rows - 1);
+                const int pos = rt.pos0 + row / a.group;
+                const int lo = key_lo(a, pos), hi = min(key_hi(a, pos, rt.kv_len), key_end);
 #pragma unroll
-                for (int j = 0; j < NT; j++)
+                for (int k = 0; k < K; k++)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) mx = fmaxf(mx, x[k][j][e]);
-        };
-        score();
+                    for (int e = 0; e < 8; e++) {
+                        const int key = (t + k) * 32 + g * 8 + e;
+                        x[k][j][e] = key >= lo && key < hi ? x[k][j][e] : -INFINITY;
+                    }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < K; k++)
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) mx = fmaxf(mx, x[k][j][e]);
         if (__any(mx > kLazy + kHead)) {
             // a larger reference: from the scores again, as x may hold them against none
 #pragma unroll
@@ -429,8 +425,17 @@ struct Wave {
                 l[j] *= f;
 #pragma unroll
                 for (int d = 0; d < ND; d++) acc[j][d] *= f;
+                // the rounded scores against M, so that its own key is at kHead: in the FMA
+                // M's rounding would remain, which for scores past 2^27 is more than an f16
+                // weight holds
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    const float c = row_scale[j] * sc[k][0], b = fmaf(row_raise[j], sc[k][0], sc[k][1]);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        x[k][j][e] = x[k][j][e] == -INFINITY ? x[k][j][e] : fmaf(s[k][j][e >> 2][e & 3], c, b) - m1 + kHead;
+                }
             }
-            score();
         }
 #pragma unroll
         for (int k = 0; k < K; k++)
