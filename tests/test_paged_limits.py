@@ -20,9 +20,9 @@ gpu = pytest.mark.gpu
 @pytest.mark.parametrize("f16", [True, False])
 @pytest.mark.parametrize("new", [1, 40])
 @pytest.mark.parametrize("sign", [1, -1])
-@pytest.mark.parametrize("k_scale", [1e4, 1e7, 1e12, 1e28])
+@pytest.mark.parametrize("k_scale", [1e4, 1e7, 1e12, 1e28, 1e33])
 def test_attention_of_scores_of_any_size(ctx, f16, new, sign, k_scale):
-    """Scores of 10^6 to 10^31, all of one sign: one key is at least a quarter ahead of
+    """Scores of 10^6 to 10^36, all of one sign: one key is at least a quarter ahead of
     all others, so the output is its value.  Its weight is a power of two and the others'
     are 0; what is left are the roundings of 1/vs, of the sum, its reciprocal and the
     product (2^-24 each) and the output's."""
@@ -42,3 +42,36 @@ def test_attention_of_scores_of_any_size(ctx, f16, new, sign, k_scale):
         want = np.repeat(want, n_q // n_kv, 0)[None]
         bound = np.abs(want) * (2.0 ** -22 + (2.0 ** -11 if f16 else 2.0 ** -24))
         assert (np.abs(got[cu[s]:cu[s + 1]] - want) <= bound).all(), s
+
+
+@gpu
+@pytest.mark.parametrize("hd,n_q,n_kv", [(128, 4, 2), (256, 8, 2), (512, 8, 1)])
+@pytest.mark.parametrize("new", [1, 2, 9])
+@pytest.mark.parametrize("every", [1, 3])
+def test_attention_of_offset_queries_over_blocks_with_an_outlier(ctx, hd, n_q, n_kv, new, every):
+    """f16 rows of q around 40 over blocks whose quants are 0 and a few +-1 beside an
+    outlier of 127 in a dim that q does not have: 128·Σq is two hundred and more times
+    the score.  `every`: other blocks between them use their whole range."""
+    rng = np.random.default_rng(hd + new)
+    page, kv = 32, [300, 41, 2500]
+    host, tables, cu = batch(rng, kv, [new] * 3, page, n_kv, hd)
+    for s in range(3):
+        for p in tables[s, ::every]:
+            if p >= 0:
+                k = np.zeros((n_kv, page, hd), np.int8)
+                at = rng.integers(1, hd, (n_kv, page, 4))
+                np.put_along_axis(k, at, rng.choice([-1, 1], at.shape).astype(np.int8), 2)
+                k[:, :, 0] = 127
+                host[0][p] = k
+                host[2][p] = 1.0
+            if every > 1:  # the others: scores of a like size
+                for o in tables[s, 1::every]:
+                    host[2][o] = 2e-3
+    q = 40 + rng.standard_normal((cu[-1], n_q, hd))
+    q[:, :, 0] = 0
+    q = q.astype(np.float16)
+    got = attend(ctx, to_pages(*host), torch.from_numpy(q).cuda(), tables, kv, cu, n_q, scale=1 / 32)
+    want, mag, cond, peak = ref.attention(q, host[0], host[2], host[1], host[3], tables, kv, cu, 0, 1 / 32)
+    bound = ref.attention_bound(want, mag, cond, peak, hd, max(kv), True)
+    worst = (np.abs(got - want) / bound).max()
+    assert worst <= 1
