@@ -441,7 +441,8 @@ int sgq_kv_gather_paged_q8(sgq_ctx *ctx, const sgq_kv_pages *pages, const int32_
  * (or graphs) that may overlap; sgq_attn_paged_workspace says how much is
  * used, with less (or NULL) the keys are split less.
  * fp32 rows are computed to fp32 accuracy (22-bit q and weights, fp32 sums);
- * f16 rows with f16 weights. */
+ * f16 rows with f16 weights.  V scales below 2^-80 weigh as 2^-80: an error below
+ * 1.1e-22 in out. */
 uint64_t sgq_attn_paged_workspace(const sgq_kv_pages *pages, uint32_t n_seqs, uint32_t n_tokens,
                                   uint32_t n_q_heads, uint32_t max_new, uint32_t max_kv);
 int sgq_attn_paged_q8(sgq_ctx *ctx, const sgq_kv_pages *pages, const void *q, uint64_t q_stride,

@@ -30,7 +30,11 @@ constexpr float kNoMax = -3.4e38f;    // the reference M before the first key: b
 // and their subnormals begin 2^20 below M.  (Two prompts of 4001 rows: 335 us;
 // with M moved at every larger score 389.)
 constexpr float kLazy = 8.f, kHead = 6.f;
-constexpr float kMinScale = 0x1p-100f;  // V scales below weigh as this one
+// V scales below this one weigh as it: an error below 127·2^-80 = 1.1e-22 in the output.
+// The sum of w/vs then stays finite whatever the number of keys (2^14·2^80·2^31),
+// also over blocks of zeros, and a weight that underflows (2^-126) has no more than
+// 2^-52·vs of that sum, vs the scale of the largest weight's block.
+constexpr float kMinScale = 0x1p-80f;
 
 struct AttnArgs {
     PagedPages pg;

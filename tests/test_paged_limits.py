@@ -75,3 +75,55 @@ def test_attention_of_offset_queries_over_blocks_with_an_outlier(ctx, hd, n_q, n
     bound = ref.attention_bound(want, mag, cond, peak, hd, max(kv), True)
     worst = (np.abs(got - want) / bound).max()
     assert worst <= 1
+
+
+@gpu
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("tokens", [300, 160_000])
+def test_attention_over_a_long_run_of_zero_blocks(ctx, f16, new, tokens):
+    """V blocks of zeros (scale 0) with scores 7.9 (log2) above the first keys', where
+    the running maximum need not move, and a last page that is not zero: the sum of
+    weights over scales stays finite."""
+    rng = np.random.default_rng(tokens + new)
+    page, n_q, n_kv, hd = 128, 2, 1, 128
+    host, tables, cu = batch(rng, [tokens], [new], page, n_kv, hd)
+    last = tables[0, (tokens - 1 - new) // page:]
+    rest = np.setdiff1d(tables[0][tables[0] >= 0], last)
+    host[1][rest], host[3][rest] = 0, 0
+    host[0][:], host[2][:] = 0, 1 / 64
+    host[0][:, :, :, 0] = 64  # scores of 7.9
+    host[0][tables[0, 0], :, :, 0] = 0
+    q = np.zeros((new, n_q, hd), np.float16 if f16 else np.float32)
+    scale = 7.9 * np.log(2)
+    q[:, :, 0] = 1
+    for split in (True, False):
+        got = attend(ctx, to_pages(*host), torch.from_numpy(q).cuda(), tables, [tokens], cu, n_q, scale=scale,
+                     split=split)
+        want, mag, cond, peak = ref.attention(q[-1:], host[0], host[2], host[1], host[3], tables, [tokens],
+                                              np.array([0, 1]), 0, scale)
+        assert np.abs(want).max() > 1e-6
+        bound = ref.attention_bound(want, mag, cond, peak, hd, tokens, f16)
+        assert (np.abs(got[-1:] - want) <= bound).all(), split
+
+
+@gpu
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("new", [1, 20])
+def test_attention_over_v_scales_to_the_smallest(ctx, f16, new):
+    """V scales from the smallest subnormal on beside ordinary ones and in requests of
+    their own, to 127*2^-80 more than the bound."""
+    rng = np.random.default_rng(new)
+    page, n_q, n_kv, hd, kv = 32, 4, 2, 128, [200, 130, 70]
+    host, tables, cu = batch(rng, kv, [new] * 3, page, n_kv, hd)
+    small = (2.0 ** rng.uniform(-149, -70, host[3].shape)).astype(np.float32)
+    for s in range(3):  # every other page, all pages, all pages at 1e-35
+        for j, p in enumerate(tables[s]):
+            if p >= 0 and (s or j % 2):
+                host[3][p] = small[p] if s < 2 else 1e-35
+    q = rng.standard_normal((cu[-1], n_q, hd)).astype(np.float16 if f16 else np.float32)
+    got = attend(ctx, to_pages(*host), torch.from_numpy(q).cuda(), tables, kv, cu, n_q)
+    want, mag, cond, peak = ref.attention(q, host[0], host[2], host[1], host[3], tables, kv, cu, 0, hd ** -0.5)
+    bound = ref.attention_bound(want, mag, cond, peak, hd, max(kv), f16) + 127 * 2.0 ** -80
+    # log2 of a V scale (|log2| <= 80) is rounded to 2^-18 at most, as a factor 2^-18
+    assert (np.abs(got - want) <= bound + mag * 2.0 ** -17).all()
