@@ -1114,10 +1114,10 @@ int best_parts(int units, int keys, int area) {
 Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f16, int max_new, int max_kv) {
     const int group = n_q / n_kv;
     Layout y{};
-    // requests with many rows exist only if max_new says so; a lone request
-    // needs one kernel
+    // requests with many rows exist only if max_new says so, with few only if a token's
+    // heads are few; a lone request needs one kernel
     y.many = (long long)max_new * group > kFewRows;
-    y.few = !y.many || n_seqs > 1;
+    y.few = !y.many || (n_seqs > 1 && group <= kFewRows);
     y.few_splits = 1;
     y.many_bm = 1;
     if (y.few) {
@@ -1128,8 +1128,9 @@ Layout layout(int n_tokens, int n_seqs, int n_q, int n_kv, int head_dim, bool f1
         y.many_bm = head_dim == 128   ? (f16 ? Many<_Float16, 128>::kRows : Many<float, 128>::kRows)
                     : head_dim == 256 ? (f16 ? Many<_Float16, 256>::kRows : Many<float, 256>::kRows)
                                       : (f16 ? Many<_Float16, 512>::kRows : Many<float, 512>::kRows);
-        // a request with many rows has more than kFewRows, and a last tile that is not full
-        const int last = y.few ? (int)std::min<long long>(n_seqs, (long long)n_tokens * group / (kFewRows + 1)) : 1;
+        // a request with many rows has more than kFewRows (alone it has any number), and a
+        // last tile that is not full
+        const int last = n_seqs > 1 ? (int)std::min<long long>(n_seqs, (long long)n_tokens * group / (kFewRows + 1)) : 1;
         y.many_tiles = (int)((long long)n_tokens * group / y.many_bm) + std::max(last, 1);
         // The remainder of a lone request is known, and so are its parts.  Of several it
         // is n_kv at least: no room (and no join) where even that is not worth a cut.

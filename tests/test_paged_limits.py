@@ -127,3 +127,39 @@ def test_attention_over_v_scales_to_the_smallest(ctx, f16, new):
     bound = ref.attention_bound(want, mag, cond, peak, hd, max(kv), f16) + 127 * 2.0 ** -80
     # log2 of a V scale (|log2| <= 80) is rounded to 2^-18 at most, as a factor 2^-18
     assert (np.abs(got - want) <= bound + mag * 2.0 ** -17).all()
+
+
+@gpu
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("hd,n_q,n_kv", [(128, 64, 1), (128, 34, 2), (256, 20, 1), (512, 32, 1)])
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [1, 0, 5, 30]])
+@pytest.mark.parametrize("room", [0, 400_000, 64 << 20])
+def test_attention_of_more_than_16_query_heads_a_kv_head(ctx, f16, hd, n_q, n_kv, new, room):
+    """A single token has more rows than the kernel of few rows takes: every request goes
+    to the other one, and the whole workspace with it."""
+    rng = np.random.default_rng(hd + n_q)
+    page, kv = 64, [2100, 3, 900, 3000]
+    kv = [max(k, n) for k, n in zip(kv, new)]
+    host, tables, cu = batch(rng, kv, new, page, n_kv, hd)
+    q = rng.standard_normal((cu[-1] + 2, n_q, hd)).astype(np.float16 if f16 else np.float32)
+    got = attend(ctx, to_pages(*host), torch.from_numpy(q).cuda(), tables, kv, cu, n_q, split=False,
+                 workspace=torch.empty(room, dtype=torch.uint8, device="cuda") if room else None)
+    want, mag, cond, peak = ref.attention(q, host[0], host[2], host[1], host[3], tables, kv, cu, 0, hd ** -0.5)
+    live = ~np.isnan(want)
+    assert (got[~live] == 7.0).all()
+    bound = ref.attention_bound(want, mag, cond, peak, hd, max(kv), f16)
+    assert (np.abs(got - want) <= bound)[live].all()
+
+
+def test_workspace_of_more_than_16_query_heads_a_kv_head():
+    """No part of it is for requests of few rows, which cannot occur: at most two rounds
+    of 256 parts of 256 rows."""
+    import sgq
+    L = sgq.lib()
+    p = _pages_struct(n_kv=1, n_pages=4096)
+    pp = C.cast(C.byref(p), C.c_void_p)
+    row = (128 + 2) * 4
+    for n_q, few in ((16, True), (17, False), (32, False), (64, False)):
+        got = L.sgq_attn_paged_workspace(pp, 64, 64, n_q, 40, 32768)
+        assert got and got % row == 0
+        assert (got // row > 512 * 256) == few, n_q
