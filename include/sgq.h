@@ -380,6 +380,8 @@ typedef struct {
 
 #define SGQ_ACT_F32 0
 #define SGQ_ACT_F16 1
+/* Added to an append's act: a block's scale grows by a quarter at least. */
+#define SGQ_APPEND_HEADROOM 0x100
 
 /* The tables of a step.  Request s has cached_lens[s] tokens in the cache and
  * gets new_lens[s] more (negative lengths count as 0, new ones above 2^22, the
@@ -414,7 +416,13 @@ int sgq_kv_pages_release(sgq_ctx *ctx, const int32_t *done, uint32_t n_seqs, uin
  * that holds the page's first slot begins the block anew with scale d (what
  * the page held is gone), any other leaves scale max(old, d), the block's
  * quants rounded to the scale when it grew.  quants = x / scale, to nearest,
- * ties to even.  An infinity or NaN in a row makes its block's scale NaN.
+ * ties to even.
+ * Each growth rounds the block's older quants anew.  That is up to half a step of the
+ * new scale each time and it adds up: rows appended one by one, each a little
+ * larger than the last, move the first values of a page of 128 by tens of steps.
+ * With act + SGQ_APPEND_HEADROOM a scale that must grow becomes
+ * max(d, 1.25 * old), which keeps every value within 2.5 steps of its block's
+ * scale however often that grows, for a scale up to 1.25 times the needed one.  An infinity or NaN in a row makes its block's scale NaN.
  * A slot named twice in a run takes the later row.  The rows of one page must
  * be consecutive in slot_map: two runs of one page in one call leave that
  * page's contents unspecified. */

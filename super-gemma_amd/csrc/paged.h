@@ -61,8 +61,8 @@ struct PagedPages {
     int n_pages, page_log2, n_kv, head_dim;
 };
 int launch_paged_append(hipStream_t st, const PagedPages &pg, const void *k, uint64_t k_stride,
-                        const void *v, uint64_t v_stride, bool f16, const int32_t *slots,
-                        uint32_t n_tokens);
+                        const void *v, uint64_t v_stride, bool f16, float growth,
+                        const int32_t *slots, uint32_t n_tokens);
 int launch_paged_gather(hipStream_t st, const PagedPages &pg, const int32_t *slots,
                         uint32_t n_tokens, bool f16, void *k, uint64_t k_stride, void *v,
                         uint64_t v_stride);

@@ -118,6 +118,8 @@ int sgq_kv_append_paged_q8(sgq_ctx *ctx, const sgq_kv_pages *pages, const void *
     if (!ctx || (n_tokens && (!k || !v || !slot_map)))
         return fail(SGQ_ERR_VALIDATION, "%s: NULL argument", who);
     if (int rc = check_pages(who, pages, &pg)) return rc;
+    const bool headroom = act >= 0 && (act & SGQ_APPEND_HEADROOM);
+    if (headroom) act &= ~SGQ_APPEND_HEADROOM;
     if (int rc = check_act(who, act)) return rc;
     if (int rc = check_count(who, n_tokens, pages->n_kv_heads)) return rc;
     const uint64_t width = (uint64_t)pg.n_kv * pg.head_dim;
@@ -126,7 +128,7 @@ int sgq_kv_append_paged_q8(sgq_ctx *ctx, const sgq_kv_pages *pages, const void *
     if (!n_tokens) return SGQ_OK;
     DeviceGuard dev(ctx_device(ctx));
     return launch_paged_append(ctx_stream(ctx), pg, k, k_stride, v, v_stride, act == SGQ_ACT_F16,
-                               slot_map, n_tokens);
+                               headroom ? 1.25f : 1.f, slot_map, n_tokens);
 }
 
 int sgq_kv_gather_paged_q8(sgq_ctx *ctx, const sgq_kv_pages *pages, const int32_t *slot_map,

@@ -4,11 +4,15 @@
 // of a step's slot map form at most rows/P + 2·requests of them.  Per head, with
 // d = max|x| / 127 over the run (one IEEE division):
 //   the run holds the page's slot 0    the block begins anew, scale = d
-//   else                               scale = max(old, d); when it grows, the
+//   else, d <= old                     scale = old
+//   else                               scale = max(d, growth·old), and the
 //                                      block's quants become rte(q·old/scale)
 //   quants of the run's rows           rte(x/scale), 0 where scale is 0
 // rte of the real quotient, ties to even: the fp32 product with the reciprocal
 // gives the integer up to one, and the exact residual x - t·scale decides.
+// Each growth moves the older values by up to half a step, s_i/2 of the i-th scale.
+// With s_i >= growth·s_(i-1) that is growth/(2·(growth-1)) steps of the last together at
+// most; with growth 1, as many halves as there were.
 // A row with an infinity or a NaN makes the scale NaN, so that attention over
 // the block is NaN too instead of quietly wrong.
 #include <algorithm>
@@ -116,7 +120,7 @@ __device__ __forceinline__ uint32_t most(uint32_t m, float4 x) {  // as bits: Na
 template <typename T, int HD>
 __global__ __launch_bounds__(kAppThreads) void paged_append_kernel(
     const T *__restrict__ k, uint64_t k_stride, const T *__restrict__ v, uint64_t v_stride,
-    const int32_t *__restrict__ slots, int n_tokens, int window, PagedPages pg) {
+    const int32_t *__restrict__ slots, int n_tokens, int window, float growth, PagedPages pg) {
     constexpr int U = HD / 8;    // 8-dim units of a row
     __shared__ int row_of[128];  // offset in the page -> row of the run, -1: none
     __shared__ uint32_t amax_s[kAppThreads / 64];
@@ -189,8 +193,9 @@ __global__ __launch_bounds__(kAppThreads) void paged_append_kernel(
             if (need != need || old != old) {
                 scale = __uint_as_float(0x7fc00000u);
             } else if (need > old) {
+                scale = fmaxf(need, old * growth);
                 uint4 *w = reinterpret_cast<uint4 *>(quants);
-                const float up = Grid::raise(need), d = need * up, inv = 1.f / d;
+                const float up = Grid::raise(scale), d = scale * up, inv = 1.f / d;
                 for (int i = tid; i < (HD << lg) / 16; i += kAppThreads) w[i] = regrid(w[i], old * up, d, inv);
                 __syncthreads();  // the run's quants go over the old ones
             } else {
@@ -316,7 +321,7 @@ __global__ __launch_bounds__(kAppThreads) void paged_gather_kernel(
 
 template <typename T, int HD>
 int append(hipStream_t st, const PagedPages &pg, const void *k, uint64_t k_stride, const void *v,
-           uint64_t v_stride, const int32_t *slots, int n) {
+           uint64_t v_stride, float growth, const int32_t *slots, int n) {
     // Single tokens want a workgroup each (16 heads of 128, 64 requests: 16 us with windows
     // of 1, 24 of 8, 59 of 32), runs as few empty workgroups as possible (a prompt of
     // 2040 rows: 56 us of 1, 34 of 8, 27 of 32; 4096 rows: 42 of 63, 53 of 32).  Many
@@ -326,7 +331,7 @@ int append(hipStream_t st, const PagedPages &pg, const void *k, uint64_t k_strid
     const dim3 grid((n + window - 1) / window * pg.n_kv, 2);
     hipLaunchKernelGGL((paged_append_kernel<T, HD>), grid, dim3(kAppThreads), 0, st,
                        static_cast<const T *>(k), k_stride, static_cast<const T *>(v), v_stride, slots,
-                       n, window, pg);
+                       n, window, growth, pg);
     SGQ_HIP(hipGetLastError());
     return SGQ_OK;
 }
@@ -353,9 +358,9 @@ int gather(hipStream_t st, const PagedPages &pg, const int32_t *slots, int n, vo
     return fail(SGQ_ERR_VALIDATION, "paged cache: head_dim %d unsupported", pg.head_dim)
 
 int launch_paged_append(hipStream_t st, const PagedPages &pg, const void *k, uint64_t k_stride,
-                        const void *v, uint64_t v_stride, bool f16, const int32_t *slots,
-                        uint32_t n_tokens) {
-    SGQ_BY_TYPE(append, st, pg, k, k_stride, v, v_stride, slots, (int)n_tokens);
+                        const void *v, uint64_t v_stride, bool f16, float growth,
+                        const int32_t *slots, uint32_t n_tokens) {
+    SGQ_BY_TYPE(append, st, pg, k, k_stride, v, v_stride, growth, slots, (int)n_tokens);
 }
 
 int launch_paged_gather(hipStream_t st, const PagedPages &pg, const int32_t *slots,

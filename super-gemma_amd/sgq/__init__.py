@@ -289,6 +289,7 @@ class KvPages:
 
 
 _ACT = {torch.float32: 0, torch.float16: 1}
+_APPEND_HEADROOM = 0x100
 
 
 def _i32(t, n, dev, name):
@@ -562,9 +563,12 @@ class GpuContext:
             raise ValidationError(6, f"k, v: {n} rows of one type expected")
         return kp, ks, vp, vs, _i32(slot_map, n, dev, "slot_map"), n, _ACT[k.dtype]
 
-    def kv_append_paged_q8(self, pages: KvPages, k, v, slot_map):
-        """Write the rows k, v [n, n_kv, head_dim] to their slots (sgq_kv_append_paged_q8)."""
+    def kv_append_paged_q8(self, pages: KvPages, k, v, slot_map, headroom: bool = False):
+        """Write the rows k, v [n, n_kv, head_dim] to their slots (sgq_kv_append_paged_q8).
+        headroom: a block's scale grows by a quarter at least, which bounds what the
+        older values of a page lose by being rounded again for each larger row."""
         kp, ks, vp, vs, sp, n, act = self._kv_rows(pages, k, v, slot_map)
+        act |= _APPEND_HEADROOM if headroom else 0
         _check(lib().sgq_kv_append_paged_q8(self._h, pages._p, kp, ks, vp, vs, act, sp, n))
 
     def kv_gather_paged_q8(self, pages: KvPages, slot_map, k, v):

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import _paged as ref
-from test_paged import FAKE, _pages_struct, attend, batch, from_pages, i32, refused, to_pages
+from test_paged import FAKE, _pages_struct, attend, batch, from_pages, i32, pool, refused, to_pages
 
 gpu = pytest.mark.gpu
 
@@ -163,3 +163,133 @@ def test_workspace_of_more_than_16_query_heads_a_kv_head():
         got = L.sgq_attn_paged_workspace(pp, 64, 64, n_q, 40, 32768)
         assert got and got % row == 0
         assert (got // row > 512 * 256) == few, n_q
+
+
+# ---- blocks that grow again and again ---------------------------------------------------
+
+def append_rows(q, d, x, slots, growth):
+    """One append of rows of one page, as the header has it."""
+    page = q.shape[2]
+    p, offs = slots[0] // page, [s % page for s in slots]
+    assert all(s // page == p for s in slots)
+    r = x.astype(np.float64)
+    for h in range(q.shape[1]):
+        need, old = np.float32(np.abs(r[:, h]).max() / 127.0), d[p, h]
+        if 0 in offs:
+            d[p, h] = need
+        elif need > old:
+            d[p, h] = max(need, old * np.float32(growth))
+            q[p, h] = np.rint(q[p, h].astype(np.float64) * float(old) / float(d[p, h]))
+        q[p, h, offs] = np.rint(r[:, h] / float(d[p, h]))
+
+
+def rising_rows(rng, page, n_kv, hd, rise):
+    """A page's rows, each `rise` times the size of the one before it."""
+    x = rng.uniform(-1, 1, (page, n_kv, hd)) * 0.9
+    x[:, :, 0] = 1
+    return (x * rise ** np.arange(page)[:, None, None]).astype(np.float32)
+
+
+def one_by_one(x, growth):
+    """Quants, scales and the largest |value - row| in steps after a page's rows were
+    appended one call each."""
+    page = len(x)
+    q, d = np.zeros((1, x.shape[1], page, x.shape[2]), np.int8), np.zeros((1, x.shape[1]), np.float32)
+    for i in range(page):
+        append_rows(q, d, x[i:i + 1], [i], growth)
+    back = q[0].transpose(1, 0, 2).astype(np.float64) * d[0].astype(np.float64)[None, :, None]
+    return q, d, (np.abs(back - x) / d[0][None, :, None]).max()
+
+
+def steps_lost(page):
+    """growth/(2·(growth-1)) at 1.25, and that each grown scale is an fp32 number."""
+    return 2.5 * (1 + page * 2.0 ** -23)
+
+
+@pytest.mark.parametrize("rise", [1.005, 1.02, 1.3, 1.9])
+@pytest.mark.parametrize("page", [32, 128])
+def test_headroom_bounds_what_rounding_again_loses(page, rise):
+    """The definition itself; growing as far as needed alone loses tens of steps."""
+    x = rising_rows(np.random.default_rng(page), page, 1, 128, rise)
+    assert one_by_one(x, 1.25)[2] <= steps_lost(page)
+    q, d, plain = one_by_one(x, 1.0)
+    assert plain <= page / 2
+    if rise == 1.005 and page == 128:
+        assert plain > 20
+    q1, d1 = np.zeros_like(q), np.zeros_like(d)  # without headroom: the shared plain form's rule
+    for i in range(page):
+        ref.append(q1, d1, x[i:i + 1], [i])
+    assert np.array_equal(q, q1) and np.array_equal(d, d1)
+
+
+@gpu
+@pytest.mark.parametrize("headroom", [False, True])
+@pytest.mark.parametrize("page,hd,f16", [(32, 128, False), (64, 256, True), (128, 512, False)])
+def test_rows_appended_one_by_one_stay_within_the_bound(ctx, headroom, page, hd, f16):
+    """Rising rows one call each, K and V: equal to the definition, and with headroom read
+    back within the bound of the rows that went in."""
+    import sgq
+    n_kv = 2
+    rng = np.random.default_rng(page)
+    dt = np.float16 if f16 else np.float32
+    x = [rising_rows(rng, page, n_kv, hd, r).astype(dt) for r in (1.005, 1.03)]
+    pages = sgq.KvPages.empty(3, page, n_kv, hd)
+    slots = i32(np.arange(page) + page)
+    dev = [torch.from_numpy(t).cuda() for t in x]
+    for i in range(page):
+        ctx.kv_append_paged_q8(pages, dev[0][i:i + 1], dev[1][i:i + 1], slots[i:i + 1], headroom=headroom)
+    back = torch.empty((2, page, n_kv, hd), device="cuda")
+    ctx.kv_gather_paged_q8(pages, slots, back[0], back[1])
+    kq, vq, ks, vs = from_pages(pages)
+    for got, quants, scales, rows in zip(back.double().cpu().numpy(), (kq, vq), (ks, vs), x):
+        q, d, _ = one_by_one(rows, 1.25 if headroom else 1.0)
+        assert np.array_equal(quants[1], q[0]) and np.array_equal(scales[1], d[0])
+        assert (quants[[0, 2]] == 0).all() and (scales[[0, 2]] == 0).all()
+        if headroom:  # the value is rounded once more, by 2^-24 of 127 steps
+            steps = steps_lost(page) + 127 * 2.0 ** -24
+            assert (np.abs(got - rows.astype(np.float64)) <= steps * scales[1][None, :, None]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_headroom_of_runs(ctx, dtype):
+    """Runs of several rows with headroom: blocks that begin anew, that stay, that grow by
+    less and by more than a quarter, of subnormal scales, of scale 0 and NaN."""
+    rng = np.random.default_rng(4)
+    page, n_kv, hd = 32, 2, 128
+    host = pool(rng, 9, n_kv, page, hd)
+    size = [1.0, 0.5, 1.1, 3.0, 1.0, 1.0, 1.0, 0.0]
+    for d in (host[2], host[3]):
+        d[:] = 1 / 127
+        d[4], d[5], d[6] = 1e-41, 0, np.nan
+    host[0][5] = host[1][5] = 0
+    x, slots = [], []
+    for p, s in enumerate(size):
+        first = 0 if p == 0 else 3
+        slots.append(list(range(p * page + first, p * page + first + 5)))
+        r = rng.uniform(-1, 1, (5, n_kv, hd))
+        r[1, :, 7] = 1
+        x.append((r * s).astype(dtype))
+    pages = to_pages(*host)
+    k = torch.from_numpy(np.concatenate(x)).cuda()
+    ctx.kv_append_paged_q8(pages, k, k, i32(sum(slots, [])), headroom=True)
+    for quants, scales, q, d in zip(from_pages(pages)[:2], from_pages(pages)[2:], host[:2], host[2:]):
+        for r, s in zip(x, slots):
+            if np.isnan(d[s[0] // page]).all():
+                q[6][:, 3:8] = 0
+                continue
+            append_rows(q, d, r, s, 1.25)
+        assert np.array_equal(scales, d, equal_nan=True) and np.array_equal(quants, q)
+
+
+@pytest.mark.parametrize("act", [0x102, 0x200, 0x301, -0x100, -1])
+def test_bad_append_flags_are_refused(act):
+    import sgq
+    L = sgq.lib()
+    p = _pages_struct()
+    pp = C.cast(C.byref(p), C.c_void_p)
+    refused(L.sgq_kv_append_paged_q8(FAKE, pp, FAKE, 512, FAKE, 512, act, FAKE, 3), "activation type")
+    # headroom is the append's alone
+    refused(L.sgq_kv_gather_paged_q8(FAKE, pp, FAKE, 3, 0x100, FAKE, 512, FAKE, 512), "activation type")
+    refused(L.sgq_attn_paged_q8(FAKE, pp, FAKE, 1024, 0x101, FAKE, 4, FAKE, FAKE, 2, 2, 8, 1, 99, 0, 0.1, FAKE,
+                                1024, None, 0), "activation type")
