@@ -397,7 +397,13 @@ typedef struct {
  *   missing [1]             how many tokens got no slot, or no row in slot_map
  *   n_free_out [1]          the entries left
  * kv_lens may be cached_lens and n_free_out may be n_free (a captured step
- * that advances itself).  n_seqs <= 4096. */
+ * that advances itself).  n_seqs <= 4096.
+ * A token without a page stays without one in later steps, and is not attended.
+ * After missing > 0 either undo the step - the lengths and *n_free of before
+ * together, before anything is released: the popped pages are then on the stack
+ * again - and plan again once others are released; or release the requests that ran
+ * short, at the kv_lens written here.  With the lengths alone set back the popped
+ * pages would be lost. */
 int sgq_kv_pages_plan(sgq_ctx *ctx, const int32_t *cached_lens, const int32_t *new_lens,
                       uint32_t n_seqs, uint32_t page_size, int32_t *block_tables,
                       uint32_t max_pages, const int32_t *free_list, uint32_t n_pages,

@@ -165,6 +165,86 @@ def test_workspace_of_more_than_16_query_heads_a_kv_head():
         assert (got // row > 512 * 256) == few, n_q
 
 
+# ---- pools that run out -------------------------------------------------------------------
+
+def all_pages(tables, lens, free, n_free, page):
+    """The pages in use and on the stack, each once if none is lost."""
+    used = [p for row, n in zip(tables, lens) for p in row[:min(-(-n // page), len(row))] if p >= 0]
+    return sorted([int(p) for p in used] + [int(p) for p in free[:n_free]])
+
+
+class Server:
+    """Five requests over 16 pages of 32 tokens, on the device or as the plain form."""
+    page, n, width, pool = 32, 5, 8, 16
+
+    def __init__(self, ctx=None):
+        self.ctx = ctx
+        self.lens, self.tables = [0] * self.n, np.full((self.n, self.width), -1, np.int32)
+        self.free, self.n_free = np.arange(self.pool, dtype=np.int32), self.pool
+        self.slots = None
+
+    def plan(self, new, rows=400):
+        if self.ctx is None:
+            self.tables, self.lens, _, self.slots, self.n_free, missing = ref.plan(
+                self.lens, new, self.tables, self.free, self.n_free, self.page, rows)
+            return missing
+        d = [i32(x) for x in (self.lens, new, self.tables, self.free, [self.n_free])]
+        out = [i32([0]), i32([0] * self.n), i32([0] * (self.n + 1)), i32([0] * rows), i32([0])]
+        self.ctx.kv_pages_plan(*d, *out, self.page)
+        self.tables, self.lens, self.n_free = d[2].cpu().numpy(), out[1].tolist(), out[0].item()
+        self.slots = out[3].tolist()
+        assert np.array_equal(d[3].cpu().numpy(), self.free)  # popping leaves the entries
+        return out[4].item()
+
+    def release(self, done):
+        if self.ctx is None:
+            self.lens, self.tables, self.free, self.n_free = ref.release(
+                done, self.lens, self.tables, self.free, self.n_free, self.page)
+            return
+        d = [i32(x) for x in (done, self.lens, self.tables, self.free, [self.n_free])]
+        self.ctx.kv_pages_release(*d, self.page)
+        self.lens, self.tables, self.free, self.n_free = (d[1].tolist(), d[2].cpu().numpy(), d[3].cpu().numpy(),
+                                                          d[4].item())
+
+    def whole(self):
+        return all_pages(self.tables, self.lens, self.free, self.n_free, self.page) == list(range(self.pool))
+
+
+def run_out_and_go_on(ctx):
+    for undo in (True, False):
+        s = Server(ctx)
+        assert s.plan([100, 30, 64, 1, 20]) == 0 and s.whole()  # 4 + 1 + 2 + 1 + 1 of 16
+        lens, n_free = list(s.lens), s.n_free
+        assert s.plan([1, 120, 1, 40, 90]) > 0 and s.n_free == 0  # 4 + 1 + 1 + 3, of 7
+        short = [i for i in range(s.n) if (s.tables[i, :-(-s.lens[i] // s.page)] < 0).any()]
+        assert short == [4] and (s.tables[4] >= 0).sum() == 2  # one of the three it needs
+        if undo:
+            s.lens, s.n_free = lens, n_free
+            assert s.whole()
+            s.release([0, 0, 1, 0, 0])
+            assert s.whole()
+            assert s.plan([1, 120, 0, 40, 90]) == 0 and s.whole()
+            assert s.lens == [101, 150, 0, 41, 110]
+        else:
+            assert s.whole()  # with the advanced lengths the tables hold what was popped
+            s.release([int(i in short) for i in range(s.n)])
+            assert s.whole() and s.lens[4] == 0
+            assert s.plan([1, 1, 1, 1, 33]) == 0 and s.whole()
+        live = [x for x in s.slots if x >= 0]
+        assert len(set(live)) == len(live)  # no slot of two tokens
+
+
+def test_a_pool_that_runs_out_loses_no_page_plain():
+    run_out_and_go_on(None)
+
+
+@gpu
+def test_a_pool_that_runs_out_loses_no_page(ctx):
+    """missing > 0, then either the step undone (lengths and count of free pages), others
+    released and the step planned again, or the short request released as it is."""
+    run_out_and_go_on(ctx)
+
+
 # ---- blocks that grow again and again ---------------------------------------------------
 
 def append_rows(q, d, x, slots, growth):
