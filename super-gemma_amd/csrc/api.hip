@@ -14,7 +14,7 @@
 #include <string>
 #include <vector>
 
-#include "paged.h"
+#include "sgq_internal.h"
 
 struct sgq_ctx {
     int device = 0;

@@ -15,8 +15,6 @@
 
 namespace sgq {
 
-int ctx_device(const sgq_ctx *ctx);
-
 // The calling thread's current device is the context's while one of these lives.
 class DeviceGuard {
   public:

@@ -36,6 +36,7 @@ const DeviceInfo &device_info();
 
 hipStream_t ctx_stream(const sgq_ctx *ctx);
 void *ctx_workspace(const sgq_ctx *ctx);
+int ctx_device(const sgq_ctx *ctx);
 
 // ---- kernel launchers (one per hot-path kernel family) ------------------
 // workspace: >= kGemvWorkspace bytes of device memory (x limb table), or
