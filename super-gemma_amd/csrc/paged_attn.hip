@@ -381,6 +381,8 @@ struct Wave {
                     raise_max = 128.f * sums * fabsf(row_scale[i]);
                     // an infinite or NaN row is NaN either way, and decides nothing for the others
                     if (!(raise_max < INFINITY)) raise_max = 0.f;
+                    // nor are scales near fp32's end taken times 2^24, however small Σq
+                    raise_max = fmaxf(raise_max, 0x1p-90f * fmaxf(1.f, fabsf(a.scale_log2)));
 #pragma unroll
                     for (int d = 1; d < 16; d <<= 1) raise_max = fmaxf(raise_max, __shfl_xor(raise_max, d));
                     raise_max = lane_f(raise_max, 0);  // in a scalar register

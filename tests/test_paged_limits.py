@@ -45,6 +45,34 @@ def test_attention_of_scores_of_any_size(ctx, f16, new, sign, k_scale):
 
 
 @gpu
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("k_scale", [1e20, 1e33, 1e35])
+def test_attention_of_queries_without_a_sum_over_large_k_scales(ctx, f16, new, k_scale):
+    """q of zeros weighs all keys alike; q of pairs that cancel prefers the key whose
+    quants differ most."""
+    rng = np.random.default_rng(new)
+    page, n_q, n_kv, hd, kv = 32, 4, 2, 128, [330, 130]
+    host, tables, cu = batch(rng, kv, [new, new], page, n_kv, hd)
+    host[2][:] = k_scale
+    host[0][:, :, :, ::2] = rng.integers(50, 60, host[0][:, :, :, ::2].shape)
+    host[0][:, :, :, 1::2] = rng.integers(40, 50, host[0][:, :, :, ::2].shape)
+    for s in range(2):
+        host[0][tables[s, 1], :, 7, ::2], host[0][tables[s, 1], :, 7, 1::2] = 110, 10
+    q = np.zeros((cu[-1], n_q, hd), np.float16 if f16 else np.float32)
+    q[:, 1::2, ::2], q[:, 1::2, 1::2] = 1, -1  # heads 1 and 3
+    got = attend(ctx, to_pages(*host), torch.from_numpy(q).cuda(), tables, kv, cu, n_q)
+    small = [t.copy() for t in host]
+    small[2][:] = 1  # the same softmax, to less than fp64 tells
+    want, mag, cond, peak = ref.attention(q, small[0], small[2], host[1], host[3], tables, kv, cu, 0, hd ** -0.5)
+    # exact scores (0, or apart by 10^20 and more): the weights' and sums' roundings only
+    bound = ref.attention_bound(want, mag, 0 * cond, peak, hd, max(kv), f16)
+    rows = np.concatenate([np.arange(kv[s] - new, kv[s]) for s in range(2)]) >= 39
+    assert rows.any()
+    assert (np.abs(got - want) <= bound)[:, ::2].all()
+    assert (np.abs(got - want) <= bound)[rows].all()
+
+@gpu
 @pytest.mark.parametrize("hd,n_q,n_kv", [(128, 4, 2), (256, 8, 2), (512, 8, 1)])
 @pytest.mark.parametrize("new", [1, 2, 9])
 @pytest.mark.parametrize("every", [1, 3])
