@@ -449,7 +449,11 @@ int sgq_kv_gather_paged_q8(sgq_ctx *ctx, const sgq_kv_pages *pages, const int32_
  * out [n_tokens x n_q_heads x head_dim] of q's type; a row that attends
  * nothing is 0, rows behind the last request are left as they were.
  * max_new: no request has more rows than this (rows past it are not
- * computed).  max_kv: about the longest kv_lens, by which the keys of long
+ * computed).  The launches are laid out for it: a step of single tokens passes 1.
+ * A request alone (n_seqs 1) is cut for n_tokens and max_new rows, so one that then
+ * has a single token is slow (32768 keys of 512 dims: 2.1 ms with 500, 37 us with 1),
+ * as are single tokens of more than 16 query heads a kv head, which share
+ * tiles made for many rows.  max_kv: about the longest kv_lens, by which the keys of long
  * requests are split over workgroups; any value gives the same result up to
  * rounding.  workspace: device memory for those splits, not shared by calls
  * (or graphs) that may overlap; sgq_attn_paged_workspace says how much is

@@ -67,7 +67,11 @@ __device__ __forceinline__ int clamped(int v, int lo, int hi) { return min(max(v
 // Requests with at most kFewRows rows a kv head (single tokens) share a wave's
 // 16 columns; their keys are what is spread over the GPU, and their quants go from
 // memory to registers.  Through the kernel of many rows, whose waves share keys
-// in LDS, 64 single tokens over up to 8192 keys take 624 us in place of 244.
+// in LDS, 64 single tokens over up to 8192 keys take 624 us in place of 244.  Two kinds of
+// single tokens go there all the same: those with more than 16 query heads a kv head
+// (64 of 32 heads over up to 2000 keys: 32 us), and a lone request's where max_new
+// announces more rows, as the keys are then cut for those (8191 keys of 128 dims 27 us,
+// with max_new 1 12.7; 32768 of 512 dims 2061 and 37).
 constexpr int kFewRows = 16;
 
 __device__ __forceinline__ bool request_rows(const AttnArgs &a, int seq, RowTile *t) {
@@ -489,7 +493,9 @@ struct Wave {
     // RAISED: K comes as quants_f16_raised.  STREAM: no other wave reads these pages
     // soon, so they are not kept in the caches (64 requests of up to 8192 keys, 16 heads
     // of 128: 243 us, kept 256; one of 32768: 29 and 33).  Not at 512 dims, where that
-    // is the slower way (12 requests of up to 32768, 4 heads: 197 us, kept 184).
+    // is the slower way for all but a lone request (4 heads: 12 requests of up to 32768 207 us,
+    // kept 192; 30 of up to 9000 187 and 174; 40 of up to 1000 52.5 and 50.5; 7 of up to
+    // 9000 47.5 and 46.9; one of 32768 37.1 and 39.7).
     template <bool STREAM, bool RAISED>
     __device__ __forceinline__ void attend_as(const AttnArgs &a, const RowTile &rt, TilePages &pages, int head,
                                               int t0, int t1, int step, int lane) {
@@ -710,8 +716,11 @@ __global__ __launch_bounds__(kFewWaves * 64, HD == 128 ? 3 : HD == 256 ? 2 : 1) 
 // The products of f16 rows of 128 dims have 32 rows a wave, at half the LDS reads
 // of 16 (two prompts of 4001 rows: 335 us and 440), four reads ahead (two: 356); wider
 // rows' accumulators leave no room for that.  Bound by LDS reads and the
-// scores' vector work beside the products: the prompts run at 780 - 840 TFLOP/s, 1111 fp32
-// rows of 256 dims with a window, at two products each, at 310 (620 done).
+// scores' vector work beside the products.  In TFLOP/s, f16: two prompts of 4001 rows of 128
+// dims 820, 2048 rows of 256 dims 600 and of 512 dims 411 (there each wave of 16 rows reads
+// all of K and V from LDS, and the one wave of a SIMD weighs alone).  fp32, at two
+// products each: 2048 rows of 128 dims 353 (706 done), 1111 of 256 dims with a window
+// 320 (640), 1024 of 512 dims over 2048 keys 342 (684).
 template <typename T, int HD>
 struct Many {
     static constexpr bool F32 = sizeof(T) == 4;

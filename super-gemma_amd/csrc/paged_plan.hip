@@ -12,8 +12,8 @@
 // scans both sums in LDS and pops the pages: the thread of a page (or of a row)
 // finds its request by bisection in the LDS sums.  It fills the slot map too up to
 // four rows a thread; a longer one goes to a second launch over the whole GPU
-// (64 rows: 8.4 us in one launch, 13.7 in two; 4060 rows: 27.7 and 30.5, with a
-// release; 8100: 29.2 and 29.3; 32000: 64 and 35).
+// (64 rows: 9.0 us in one launch, 11.5 in two; with a release before them and the
+// copies that it works on, 4060 rows: 30.1 and 31.6; 8100: 27.9 and 28.8; 32000: 62 and 34).
 #include "paged.h"
 
 namespace sgq {
