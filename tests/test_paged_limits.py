@@ -106,6 +106,31 @@ def test_attention_of_offset_queries_over_blocks_with_an_outlier(ctx, hd, n_q, n
 
 
 @gpu
+@pytest.mark.parametrize("hd,n_q,n_kv", [(128, 4, 2), (512, 8, 1)])
+@pytest.mark.parametrize("first", [0, 9000, 17900])
+def test_attention_of_offset_queries_where_far_blocks_decide(ctx, hd, n_q, n_kv, first):
+    """The same in an uncut request of more pages than a wave looks up at a time: only the
+    blocks of tokens first .. first + 100 have an outlier, and they carry the softmax."""
+    rng = np.random.default_rng(hd + first)
+    page, kv = 32, [18000]
+    host, tables, cu = batch(rng, kv, [1], page, n_kv, hd)
+    host[2][:] = 1e-4
+    for p in tables[0, first // page:(first + 100) // page]:
+        k = np.zeros((n_kv, page, hd), np.int8)
+        at = rng.integers(1, hd, (n_kv, page, 8))
+        np.put_along_axis(k, at, 1, 2)
+        k[:, :, 0] = 127
+        host[0][p], host[2][p] = k, 1.0
+    q = 40 + rng.standard_normal((1, n_q, hd))
+    q[:, :, 0] = 0
+    q = q.astype(np.float16)
+    got = attend(ctx, to_pages(*host), torch.from_numpy(q).cuda(), tables, kv, cu, n_q, scale=1 / 16, split=False)
+    want, mag, cond, peak = ref.attention(q, host[0], host[2], host[1], host[3], tables, kv, cu, 0, 1 / 16)
+    bound = ref.attention_bound(want, mag, cond, peak, hd, kv[0], True)
+    worst = (np.abs(got - want) / bound).max()
+    assert worst <= 1
+
+@gpu
 @pytest.mark.parametrize("f16", [True, False])
 @pytest.mark.parametrize("new", [1, 20])
 @pytest.mark.parametrize("tokens", [300, 160_000])
