@@ -428,7 +428,8 @@ int sgq_kv_pages_release(sgq_ctx *ctx, const int32_t *done, uint32_t n_seqs, uin
  * larger than the last, move the first values of a page of 128 by tens of steps.
  * With act + SGQ_APPEND_HEADROOM a scale that must grow becomes
  * max(d, 1.25 * old), which keeps every value within 2.5 steps of its block's
- * scale however often that grows, for a scale up to 1.25 times the needed one.  An infinity or NaN in a row makes its block's scale NaN.
+ * scale however often that grows, for a scale up to 1.25 times the needed one.
+ * An infinity or NaN in a row makes its block's scale NaN.
  * A slot named twice in a run takes the later row.  The rows of one page must
  * be consecutive in slot_map: two runs of one page in one call leave that
  * page's contents unspecified. */
@@ -453,9 +454,9 @@ int sgq_kv_gather_paged_q8(sgq_ctx *ctx, const sgq_kv_pages *pages, const int32_
  * A request alone (n_seqs 1) is cut for n_tokens and max_new rows, so one that then
  * has a single token is slow (32768 keys of 512 dims: 2.1 ms with 500, 37 us with 1),
  * as are single tokens of more than 16 query heads a kv head, which share
- * tiles made for many rows.  max_kv: about the longest kv_lens, by which the keys of long
- * requests are split over workgroups; any value gives the same result up to
- * rounding.  workspace: device memory for those splits, not shared by calls
+ * tiles made for many rows.
+ * max_kv: about the longest kv_lens, by which the keys of long requests are split
+ * over workgroups; any value gives the same result up to rounding.  workspace: device memory for those splits, not shared by calls
  * (or graphs) that may overlap; sgq_attn_paged_workspace says how much is
  * used, with less (or NULL) the keys are split less.
  * fp32 rows are computed to fp32 accuracy (22-bit q and weights, fp32 sums);

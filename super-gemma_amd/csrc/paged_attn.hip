@@ -227,7 +227,10 @@ __device__ __forceinline__ KeySpan key_span(const AttnArgs &a, const RowTile &rt
 }
 
 // 8 quants (two words) as f16: byte u = q + 128 under the exponent of 1024
-// makes 1024 + u exactly, minus 1152 is q.
+// makes 1024 + u exactly, minus 1152 is q.  (As the subnormal u·2^-24, with 128·Σq taken
+// from the scores, 4 of the 10 operations go: 30 single tokens over up to 9000 keys of 512
+// dims 174 us for 177, of other dims the same.  But where q has a mean and a block's quants
+// are small beside an outlier, that term is far larger than the scores and takes their digits.)
 __device__ __forceinline__ h8 quants_f16(uint32_t w0, uint32_t w1) {
     const uint32_t x0 = w0 ^ 0x80808080u, x1 = w1 ^ 0x80808080u, e = 0x64646464u;
     const uint32_t p[4] = {__builtin_amdgcn_perm(e, x0, 0x04010400u),
@@ -245,16 +248,6 @@ __device__ __forceinline__ h8 quants_f16(uint32_t w0, uint32_t w1) {
     return r;
 }
 
-// 8 quants as the f16 numbers (q + 128)·2^-24: the byte is a subnormal's bits.
-// Exact, at 6 operations in place of 10; who takes these subtracts the 128, where that
-// leaves the score's digits (Wave::raise_max).
-__device__ __forceinline__ h8 quants_f16_raised(uint32_t w0, uint32_t w1) {
-    const uint32_t x0 = w0 ^ 0x80808080u, x1 = w1 ^ 0x80808080u;
-    const uint4 p = make_uint4(__builtin_amdgcn_perm(0, x0, 0x0c010c00u), __builtin_amdgcn_perm(0, x0, 0x0c030c02u),
-                               __builtin_amdgcn_perm(0, x1, 0x0c010c00u), __builtin_amdgcn_perm(0, x1, 0x0c030c02u));
-    return __builtin_bit_cast(h8, p);
-}
-
 __device__ __forceinline__ float lane_f(float v, int lane) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
@@ -266,10 +259,14 @@ __device__ __forceinline__ V load(const int8_t *p) {
 }
 
 // The pages of 64 tiles and what their scales make of the scores: one tile a lane,
-// read lane by lane.
+// read lane by lane.  LEAN keeps the V scale and takes its log2 and reciprocal tile by
+// tile, a register less: with it single f16 tokens of 512 dims spill nothing in their loop
+// (30 of up to 9000 keys 177 us, else 185).  The loop of many rows, bound by vector work, is
+// faster without (2048 f16 rows of 512 dims 336 us, else 350).
+template <bool LEAN>
 struct TilePages {
     int page;            // 0 where there is none
-    float ks, lv, rv;    // K scale; log2 and reciprocal of the V scale
+    float ks, lv, rv;    // K scale; log2 and reciprocal of the V scale (LEAN: lv is the scale)
     // Lane i: tile t + i·step, if that is below t1.
     __device__ __forceinline__ void load(const AttnArgs &a, const int32_t *table, int head, int t, int step, int t1) {
         const int mine = t + (threadIdx.x & 63) * step;
@@ -280,11 +277,22 @@ struct TilePages {
         const float raw = a.pg.vs[b];
         const float vs = fmaxf(raw, kMinScale) + (raw - raw);  // NaN stays
         ks = ok ? a.pg.ks[b] : 0.f;
-        lv = ok ? __builtin_amdgcn_logf(vs) : -INFINITY;  // no page: no weight
-        rv = ok && vs == vs ? 1.f / vs : 1.f;             // finite: a masked key's 0·rv stays 0
+        if constexpr (LEAN) {
+            lv = ok ? vs : 0.f;
+        } else {
+            lv = ok ? __builtin_amdgcn_logf(vs) : -INFINITY;  // no page: no weight
+            rv = ok && vs == vs ? 1.f / vs : 1.f;             // finite: a masked key's 0·rv stays 0
+        }
     }
-    __device__ __forceinline__ void scales(int lane, float (&sc)[4]) const {
-        sc[0] = lane_f(ks, lane), sc[1] = lane_f(lv, lane), sc[2] = lane_f(rv, lane), sc[3] = 0.f;
+    __device__ __forceinline__ void scales(int lane, float (&sc)[3]) const {
+        sc[0] = lane_f(ks, lane);
+        if constexpr (LEAN) {
+            const float vs = lane_f(lv, lane);
+            sc[1] = __builtin_amdgcn_logf(vs);                     // of 0: -infinity
+            sc[2] = __builtin_amdgcn_rcpf(fmaxf(vs, kMinScale));  // of a NaN or 0: finite, as above
+        } else {
+            sc[1] = lane_f(lv, lane), sc[2] = lane_f(rv, lane);
+        }
     }
 };
 
@@ -307,24 +315,10 @@ struct Wave {
     static constexpr int NC = HD / 64, ND = HD / 16;
     h8 qa[NT][NC][2], ql[F32 ? NT : 1][F32 ? NC : 1][2];
     h8 (*ql_s)[64];  // fp32 rows of 512 dims, few: ql [fragment][lane] in LDS
-    float row_scale[NT];
-    // f16 rows of few meet K raised by 128, as (q + 128)·2^-24: the score is
-    // x = (s·2^24)·(row_scale·ks) + row_raise·ks, whose second term takes 128·Σq away.
-    // The sums on the way to s lie within raise_max·ks of zero plus the score, raise_max =
-    // 128·|scale|·Σ|Σq| over runs of 8 dims, and are rounded some 20 times to 2^-24 of
-    // that; a wave takes its tiles raised if raise_max·ks <= kRaise for all of them: those
-    // roundings then add up to some 2^-13 (20 of one sign to 2^-11), below an f16 weight's.
-    // Ordinary q of zero mean are far inside (normal q of 1.5 against a scale of 0.03: 26 at
-    // 128 dims, 53 at 512).  Elsewhere, where q has a mean and the block's quants
-    // are small beside an outlier, the quants come as they are.  (Chosen tile by tile
-    // the two ways to multiply spilled at 512 dims: 200 us for 191.)
-    float row_raise[NT], raise_max;
-    static constexpr float kRaise = 512.f;
+    float row_scale[NT];  // of the scores, in log2 units
     f4 acc[NT][ND];
     float M[NT], l[NT];
 
-    // RAISED: K will come as quants_f16_raised.
-    template <bool RAISED>
     __device__ __forceinline__ void load_q(const AttnArgs &a, const RowTile &rt, int head, int n, int g) {
 #pragma unroll
         for (int i = 0; i < NT; i++) {
@@ -332,7 +326,6 @@ struct Wave {
             const T *src = static_cast<const T *>(a.q) + (size_t)(rt.tok0 + row / a.group) * a.q_stride +
                            (size_t)(head * a.group + row % a.group) * HD + g * 16;
             row_scale[i] = a.scale_log2;
-            row_raise[i] = 0.f;
             M[i] = kNoMax;
             l[i] = 0.f;
 #pragma unroll
@@ -365,32 +358,10 @@ struct Wave {
                             ql[i][c][h][j] = (_Float16)(v - (float)hi16);
                         }
             } else {
-                float sum = 0.f, sums = 0.f;
 #pragma unroll
                 for (int c = 0; c < NC; c++)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        qa[i][c][h] = *reinterpret_cast<const h8 *>(src + c * 64 + h * 8);
-                        float run = 0.f;
-#pragma unroll
-                        for (int j = 0; j < 8; j++) run += (float)qa[i][c][h][j];
-                        sum += run;
-                        sums += fabsf(run);
-                    }
-                if constexpr (RAISED) {
-                    static_assert(NT == 1, "one raise_max");
-                    sum += __shfl_xor(sum, 16), sums += __shfl_xor(sums, 16);
-                    sum += __shfl_xor(sum, 32), sums += __shfl_xor(sums, 32);
-                    row_raise[i] = -128.f * sum * row_scale[i];
-                    raise_max = 128.f * sums * fabsf(row_scale[i]);
-                    // an infinite or NaN row is NaN either way, and decides nothing for the others
-                    if (!(raise_max < INFINITY)) raise_max = 0.f;
-                    // nor are scales near fp32's end taken times 2^24, however small Σq
-                    raise_max = fmaxf(raise_max, 0x1p-90f * fmaxf(1.f, fabsf(a.scale_log2)));
-#pragma unroll
-                    for (int d = 1; d < 16; d <<= 1) raise_max = fmaxf(raise_max, __shfl_xor(raise_max, d));
-                    raise_max = lane_f(raise_max, 0);  // in a scalar register
-                }
+                    for (int h = 0; h < 2; h++) qa[i][c][h] = *reinterpret_cast<const h8 *>(src + c * 64 + h * 8);
             }
         }
     }
@@ -398,10 +369,10 @@ struct Wave {
     // The weights w (fp32 rows: w + wl) of K tiles from t on from their scores, with l,
     // and with M and acc where the reference has to move.  edge: some row does not
     // attend all keys; keys from key_end on are not this part's.  sc: each tile's K
-    // scale for s, log2 and reciprocal of its V scale, K scale for row_raise.
+    // scale, log2 and reciprocal of its V scale.
     template <int K>
     __device__ __forceinline__ void weigh(const AttnArgs &a, const RowTile &rt, int t, bool edge, int key_end,
-                                          const float (&sc)[K][4], const f4 (&s)[K][NT][2], h8 (&w)[K][NT],
+                                          const float (&sc)[K][3], const f4 (&s)[K][NT][2], h8 (&w)[K][NT],
                                           h8 (&wl)[K][F32 ? NT : 1], int n, int g) {
         float x[K][NT][8], mx = -INFINITY;
 #pragma unroll
@@ -409,7 +380,7 @@ struct Wave {
 #pragma unroll
             for (int j = 0; j < NT; j++) {
                 const float c = row_scale[j] * sc[k][0];
-                const float b = fmaf(row_raise[j], sc[k][3], sc[k][1] + (kHead - M[j]));
+                const float b = sc[k][1] + (kHead - M[j]);
 #pragma unroll
                 for (int e = 0; e < 8; e++) x[k][j][e] = fmaf(s[k][j][e >> 2][e & 3], c, b);
             }
@@ -442,7 +413,7 @@ struct Wave {
                 float m = -INFINITY;
 #pragma unroll
                 for (int k = 0; k < K; k++) {
-                    const float c = row_scale[j] * sc[k][0], b = fmaf(row_raise[j], sc[k][3], sc[k][1]);
+                    const float c = row_scale[j] * sc[k][0], b = sc[k][1];
 #pragma unroll
                     for (int e = 0; e < 8; e++)
                         m = fmaxf(m, x[k][j][e] == -INFINITY ? x[k][j][e] : fmaf(s[k][j][e >> 2][e & 3], c, b));
@@ -457,7 +428,7 @@ struct Wave {
                 // weight holds
 #pragma unroll
                 for (int k = 0; k < K; k++) {
-                    const float c = row_scale[j] * sc[k][0], b = fmaf(row_raise[j], sc[k][3], sc[k][1]);
+                    const float c = row_scale[j] * sc[k][0], b = sc[k][1];
 #pragma unroll
                     for (int e = 0; e < 8; e++)
                         x[k][j][e] = x[k][j][e] == -INFINITY ? x[k][j][e] : fmaf(s[k][j][e >> 2][e & 3], c, b) - m1 + kHead;
@@ -489,21 +460,21 @@ struct Wave {
         }
     }
 
-    // Tiles t0, t0 + step, ... below t1, of which the first 64 are in `pages`.
-    // RAISED: K comes as quants_f16_raised.  STREAM: no other wave reads these pages
+    // Tiles t0, t0 + step, ... below t1.  STREAM: no other wave reads these pages
     // soon, so they are not kept in the caches (64 requests of up to 8192 keys, 16 heads
     // of 128: 243 us, kept 256; one of 32768: 29 and 33).  Not at 512 dims, where that
     // is the slower way for all but a lone request (4 heads: 12 requests of up to 32768 207 us,
     // kept 192; 30 of up to 9000 187 and 174; 40 of up to 1000 52.5 and 50.5; 7 of up to
     // 9000 47.5 and 46.9; one of 32768 37.1 and 39.7).
-    template <bool STREAM, bool RAISED>
-    __device__ __forceinline__ void attend_as(const AttnArgs &a, const RowTile &rt, TilePages &pages, int head,
-                                              int t0, int t1, int step, int lane) {
+    template <bool STREAM>
+    __device__ __forceinline__ void attend(const AttnArgs &a, const RowTile &rt, int head, int t0, int t1,
+                                           int step, int lane) {
         const int n = lane & 15, g = lane >> 4;
         // tiles inside [all_lo, all_hi] need no mask
         const int all_lo = key_lo(a, last_pos(a, rt)), all_hi = key_hi(a, first_pos(a, rt), rt.kv_len);
         const int32_t *table = a.tables + (size_t)rt.seq * a.max_pages;
         const int lg = a.pg.page_log2;
+        TilePages<HD == 512> pages;
         const size_t lane_k = (size_t)((n >> 2) * 8 + (n & 3)) * HD + g * 16;
         const size_t lane_v = n * 32 + g * 8;
         const auto block = [&](int t, int i) {  // the quants of tile t, the wave's i-th
@@ -519,6 +490,8 @@ struct Wave {
 #pragma unroll
                 for (int h = 0; h < 2; h++) kr[c][h] = load<STREAM, u4>(p + c * 64 + h * 4 * HD);
         };
+        if (t0 >= t1) return;
+        pages.load(a, table, head, t0, step, t1);
         size_t blk = block(t0, 0);
         load_k(blk);
         // One tile.  Its V and then the next tile's K are on their way while it is
@@ -529,7 +502,7 @@ struct Wave {
             else return ql[j][c][e];
         };
         const auto tile = [&](int i, int t, auto more) {
-            float sc[1][4];
+            float sc[1][3];
             pages.scales(i % 64, sc[0]);
             const int8_t *vp = a.pg.vq + blk + lane_v;
 #pragma unroll
@@ -541,8 +514,7 @@ struct Wave {
             for (int c = 0; c < NC; c++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const h8 k0 = RAISED ? quants_f16_raised(kr[c][h].x, kr[c][h].y) : quants_f16(kr[c][h].x, kr[c][h].y);
-                    const h8 k1 = RAISED ? quants_f16_raised(kr[c][h].z, kr[c][h].w) : quants_f16(kr[c][h].z, kr[c][h].w);
+                    const h8 k0 = quants_f16(kr[c][h].x, kr[c][h].y), k1 = quants_f16(kr[c][h].z, kr[c][h].w);
 #pragma unroll
                     for (int j = 0; j < NT; j++) {
                         s[j][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qa[j][c][0], s[j][h], 0, 0, 0);
@@ -561,7 +533,6 @@ struct Wave {
                 blk = block(t + step, i + 1);
                 load_k(blk);
             }
-            if constexpr (RAISED) sc[0][3] = sc[0][0], sc[0][0] *= 0x1p24f;
             h8 wk[1][NT], wlk[1][F32 ? NT : 1], (&w)[NT] = wk[0], (&wl)[F32 ? NT : 1] = wlk[0];
             weigh<1>(a, rt, t, t * 32 < all_lo || t * 32 + 32 > all_hi, INT32_MAX, sc, sk, wk, wlk, n, g);
 #pragma unroll
@@ -577,28 +548,6 @@ struct Wave {
         int i = 0, t = t0;
         for (; t + step < t1; i++, t += step) tile(i, t, std::true_type{});
         tile(i, t, std::false_type{});
-    }
-
-    // Tiles t0, t0 + step, ... below t1.
-    template <bool STREAM>
-    __device__ __forceinline__ void attend(const AttnArgs &a, const RowTile &rt, int head, int t0, int t1,
-                                           int step, int lane) {
-        if (t0 >= t1) return;
-        const int32_t *table = a.tables + (size_t)rt.seq * a.max_pages;
-        TilePages pages;
-        bool raised = false;
-        if constexpr (!F32) {
-            raised = true;
-            for (int t = t0 + 64 * step; t < t1; t += 64 * step) {
-                pages.load(a, table, head, t, step, t1);
-                raised = raised && !__any(raise_max * pages.ks > kRaise);
-            }
-        }
-        pages.load(a, table, head, t0, step, t1);
-        // (a NaN scale decides nothing: who attends that block is NaN either way)
-        raised = raised && !__any(raise_max * pages.ks > kRaise);
-        if (!F32 && raised) attend_as<STREAM, !F32>(a, rt, pages, head, t0, t1, step, lane);
-        else attend_as<STREAM, false>(a, rt, pages, head, t0, t1, step, lane);
         finish();
     }
 };
@@ -632,7 +581,10 @@ __global__ __launch_bounds__(kFewWaves * 64, HD == 128 ? 3 : HD == 256 ? 2 : 1) 
     constexpr int CW = HD == 512 ? 256 : 128;
     __shared__ float ml_s[kFewWaves][2][16];
     __shared__ __align__(16) float o_s[kFewWaves][16][CW + 4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    // 512 dims: in a scalar register, and so are its tiles and their addresses (30 f16 tokens
+    // of up to 9000 keys 177 us, else 181; 200 of 2000 of 128 dims 187, else 184)
+    const int wave = HD == 512 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : threadIdx.x >> 6;
     // the heads of a page lie side by side, and so do their workgroups
     const int head = blockIdx.x % a.pg.n_kv, unit = blockIdx.x / a.pg.n_kv;
     const int split = unit % a.few_splits;
@@ -642,7 +594,7 @@ __global__ __launch_bounds__(kFewWaves * 64, HD == 128 ? 3 : HD == 256 ? 2 : 1) 
     if (split >= ks.parts) return;
     const int t0 = ks.t0 + split * ks.per, t1 = min(t0 + ks.per, ks.t1);
     Wave<T, HD, 1> w;
-    w.template load_q<true>(a, rt, head, n, g);
+    w.load_q(a, rt, head, n, g);
     if constexpr (Wave<T, HD, 1>::F32 && HD == 512) {
         // both halves of q, the accumulator and a tile on its way are more registers than
         // a wave has (84 spilled): the waves' common low half from LDS, 174 -> 119 us
@@ -774,7 +726,7 @@ __global__ __launch_bounds__((Many<T, HD>::kThreads), (Many<T, HD>::kWaves / 4))
     wt.rows = idle ? 1 : min(rt.rows - wave * NT * 16, NT * 16);
     const int all_lo = key_lo(a, last_pos(a, wt)), all_hi = min(key_hi(a, first_pos(a, wt), rt.kv_len), t1 * 32);
     Wave<T, HD, NT> w;
-    w.template load_q<false>(a, wt, head, n, g);
+    w.load_q(a, wt, head, n, g);
 
     const int32_t *table = a.tables + (size_t)rt.seq * a.max_pages;
     const int lg = a.pg.page_log2 - 5;  // tiles of a page, log2
@@ -923,12 +875,12 @@ __global__ __launch_bounds__((Many<T, HD>::kThreads), (Many<T, HD>::kWaves / 4))
         }
         return;
     }
-    TilePages tiles;
+    TilePages<false> tiles;
     // Steps that a wave's rows do not reach weigh nothing, like the copies past the end.
     for (int t = 0; t < steps; t++) {
         const int at = t0 + t * KT, turn = t * KT % 64;
         if (turn == 0) tiles.load(a, table, head, at, 1, t1);
-        float sc[KT][4];
+        float sc[KT][3];
 #pragma unroll
         for (int k = 0; k < KT; k++) tiles.scales(turn + k, sc[k]);
         w.template weigh<KT>(a, wt, at, at * 32 < all_lo || (at + KT) * 32 > all_hi, t1 * 32, sc, s, hi, lo, n, g);

@@ -108,9 +108,9 @@ def test_attention_of_offset_queries_over_blocks_with_an_outlier(ctx, hd, n_q, n
 @gpu
 @pytest.mark.parametrize("hd,n_q,n_kv", [(128, 4, 2), (512, 8, 1)])
 @pytest.mark.parametrize("first", [0, 9000, 17900])
-def test_attention_of_offset_queries_where_far_blocks_decide(ctx, hd, n_q, n_kv, first):
-    """The same in an uncut request of more pages than a wave looks up at a time: only the
-    blocks of tokens first .. first + 100 have an outlier, and they carry the softmax."""
+def test_attention_of_offset_queries_over_a_long_request(ctx, hd, n_q, n_kv, first):
+    """The same in an uncut request of more pages than a wave looks up at a time, of which
+    only those of tokens first .. first + 100 have an outlier."""
     rng = np.random.default_rng(hd + first)
     page, kv = 32, [18000]
     host, tables, cu = batch(rng, kv, [1], page, n_kv, hd)
