@@ -218,6 +218,30 @@ def test_workspace_of_more_than_16_query_heads_a_kv_head():
         assert (got // row > 512 * 256) == few, n_q
 
 
+@gpu
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("hd,n_q,n_kv", [(128, 8, 4), (256, 8, 2), (512, 8, 1)])
+def test_attention_of_drafts_beside_a_nan_block_a_missing_page_and_a_zero_one(ctx, f16, hd, n_q, n_kv):
+    """Two tokens of which the second begins a page: a NaN scale there is the second row's
+    alone, and a page that is missing or zero weighs as it should, at every head_dim."""
+    rng = np.random.default_rng(hd)
+    page, kv = 32, [129, 97, 65]
+    host, tables, cu = batch(rng, kv, [2, 2, 2], page, n_kv, hd)
+    tables[1, 1] = -1
+    host[1][tables[2, 0]], host[3][tables[2, 0]] = 0, 0
+    q = rng.standard_normal((cu[-1], n_q, hd)).astype(np.float16 if f16 else np.float32)
+    args = (torch.from_numpy(q).cuda(), tables, kv, cu, n_q)
+    got = attend(ctx, to_pages(*host), *args)
+    want, mag, cond, peak = ref.attention(q, host[0], host[2], host[1], host[3], tables, kv, cu, 0, hd ** -0.5)
+    assert (np.abs(got - want) <= ref.attention_bound(want, mag, cond, peak, hd, max(kv), f16)).all()
+    for d in (host[2], host[3]):
+        keep = d.copy()
+        for s in range(3):
+            d[tables[s, (kv[s] - 1) // page]] = np.nan
+        bad = attend(ctx, to_pages(*host), *args)
+        d[:] = keep
+        assert np.isnan(bad[1::2]).all() and np.array_equal(bad[::2], got[::2])
+
 # ---- pools that run out -------------------------------------------------------------------
 
 def all_pages(tables, lens, free, n_free, page):
